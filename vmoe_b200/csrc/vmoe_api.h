@@ -189,6 +189,42 @@ VMOE_API int vmoe_xent(int32_t kind, const void* logits, const void* labels, int
                        float* loss, void* dlogits, int64_t rows, int64_t n, int64_t ld,
                        int64_t ld_labels, float grad_scale, vmoe_stream_t stream);
 
+// ----------------------------------------------------------------------------- distillation
+// dtype codes of logits and values: 0 fp32, 1 bf16, 2 fp16.
+// The k <= 256 largest logits of every row, sorted (ties: lower class first; NaN above +inf):
+// values (rows, k) in the logits' type, indices (rows, k), and rest (rows) = log-sum-exp of
+// logits / temperature over all the other classes (-inf when there are none).
+VMOE_API int64_t vmoe_top_logits_max_classes(int32_t dtype);
+VMOE_API int vmoe_top_logits(const void* logits, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
+                             int64_t k, double temperature, void* values, int32_t* indices,
+                             float* rest, vmoe_stream_t stream);
+// loss (rows, fp32) = temperature^2 * KL(teacher || student) over the kept classes and, when rest is
+// set, "any other class" as one more outcome; the teacher's distribution is the softmax of
+// values / temperature (and rest). Entries whose index lies outside 0 .. n - 1 are left out, of a
+// class listed twice the first entry counts. stats (rows, 2) and slopes (rows, k), fp32, are kept
+// for the backward pass, which writes grad (rows, ld_grad) = d loss / d logits * d_loss in the
+// logits' type; columns n .. n_pad - 1 get zeros. grad rows must have the logits rows' alignment
+// within 16 bytes. d_loss_stride 0: one value for all rows.
+typedef struct VmoeDistillArgs {
+  const void* logits;
+  const void* values;
+  const void* indices;
+  const float* rest;  // may be NULL
+  float* loss;
+  float* stats;
+  float* slopes;
+  int64_t rows, n, k;
+  int64_t ld, ld_values, ld_indices;  // row strides in elements
+  double temperature;
+  int32_t dtype, values_dtype;
+  int32_t indices_wide;               // 0: int32, 1: int64
+} VmoeDistillArgs;
+VMOE_API int64_t vmoe_distill_max_classes(void);
+VMOE_API int vmoe_distill_fwd(const VmoeDistillArgs* args, vmoe_stream_t stream);
+VMOE_API int vmoe_distill_bwd(const VmoeDistillArgs* args, const float* d_loss,
+                              int64_t d_loss_stride, void* grad, int64_t ld_grad, int64_t n_pad,
+                              vmoe_stream_t stream);
+
 // ----------------------------------------------------------------------------- optimizer
 // Flat fp32 buffers of n elements (n % 1024 == 0); meta has one {weight_decay, lr_mult,
 // grad_scale, pad} float4 per 1024 elements. sums: double[3] = {sum g^2, sum update^2,

@@ -80,6 +80,20 @@ class PushArgs(ctypes.Structure):
   ]
 
 
+class DistillArgs(ctypes.Structure):
+  """Mirror of ``VmoeDistillArgs``."""
+  _fields_ = [
+      ("logits", ctypes.c_void_p), ("values", ctypes.c_void_p), ("indices", ctypes.c_void_p),
+      ("rest", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("stats", ctypes.c_void_p),
+      ("slopes", ctypes.c_void_p),
+      ("rows", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+      ("ld", ctypes.c_int64), ("ld_values", ctypes.c_int64), ("ld_indices", ctypes.c_int64),
+      ("temperature", ctypes.c_double),
+      ("dtype", ctypes.c_int32), ("values_dtype", ctypes.c_int32),
+      ("indices_wide", ctypes.c_int32),
+  ]
+
+
 def available() -> bool:
   return os.path.exists(LIB_PATH)
 
@@ -96,6 +110,8 @@ def lib() -> ctypes.CDLL:
             f"{LIB_PATH} not found: run `python -m vmoe_b200.build` (needs nvcc)")
       l = ctypes.CDLL(LIB_PATH)
       l.vmoe_last_error.restype = ctypes.c_char_p
+      l.vmoe_top_logits_max_classes.restype = ctypes.c_int64
+      l.vmoe_distill_max_classes.restype = ctypes.c_int64
       _lib = l
   return _lib
 
@@ -114,3 +130,13 @@ def ptr(t) -> int | None:
 def stream_ptr() -> int:
   import torch
   return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(t):
+  """Context in which the launches for ``t`` go to its device and to that device's current
+  stream (a no-op when that device is the current one already)."""
+  import contextlib
+  import torch
+  if t.device.index == torch.cuda.current_device():
+    return contextlib.nullcontext()
+  return torch.cuda.device(t.device)
