@@ -1,0 +1,714 @@
+// Gated MLP on tcgen05: both projections, the activation and the product in one kernel, and the
+// matching backward kernel.
+//
+//   forward   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u
+//             for training also  a = act(g)  and  s = u act'(g)
+//   backward  dh = dy Wo,  dg = dh s,  du = dh a   (and the column sums of both)
+//
+// Both are persistent warp-specialised GEMMs (TMA -> 128B-swizzled shared memory -> tcgen05.mma ->
+// TMEM -> epilogue warps), with one CTA per 128-row tile or CTA pairs on 256-row tiles, like the
+// plain GEMM of this library. Forward: the 256 accumulator columns of a tile are 128 gate columns
+// and the 128 up columns of the same hidden units, so a thread of the epilogue finds both factors
+// of its products in its own TMEM lane; in a CTA pair the even CTA stages the gate's rows of the
+// weights and the odd CTA the up projection's. Backward: the saved factors come in by TMA, one
+// 32 x 32 tile ahead of their use, and the epilogue is two products.
+//
+// Saving a and s (rounded once from fp32) instead of g and u leaves one rounding in each factor and
+// no transcendental function in the backward pass; the traffic is the same. dg and du are rounded
+// to bf16 because they are tensor-core operands of the next two GEMMs.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "ptx_sm100.cuh"
+#include "tma_host.h"
+#include "vmoe_api.h"
+
+namespace vmoe {
+
+void set_error(const char* fmt, const char* a, int code);
+int make_bf16_map(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t rows, uint64_t batch,
+                  uint64_t ld_elems, uint64_t batch_stride_elems, uint32_t box_rows,
+                  uint32_t box_inner, CUtensorMapSwizzle swizzle);
+
+namespace {
+
+constexpr int BM = 128;
+constexpr int BN = 256;
+constexpr int HALF = BN / 2;
+constexpr int BK = 64;
+constexpr int UMMA_K = 16;
+constexpr int A_BYTES = BM * BK * 2;        // 16 KiB
+constexpr int B_BYTES = BN * BK * 2;        // 32 KiB
+constexpr int CHUNK_BYTES = 64 * BK * 2;    // one 64 x 64 MN-major box
+constexpr int STAGES = 3;                   // one CTA: 48 KiB per stage
+constexpr int STAGES_PAIR = 5;              // pairs stage half of B per CTA: 32 KiB per stage
+constexpr int TMEM_COLS = 512;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int TILE_BYTES = 32 * 32 * 2;     // one staging tile: 32 rows of 64 bytes, 64B swizzle
+constexpr int EPI_TILES = 4;                // per epilogue warp
+constexpr int PIPE_BYTES = STAGES_PAIR * (A_BYTES + B_BYTES / 2);
+constexpr int SMEM_BYTES = PIPE_BYTES + EPI_WARPS * EPI_TILES * TILE_BYTES + 1024 + 256;
+static_assert(STAGES * (A_BYTES + B_BYTES) <= PIPE_BYTES, "both modes share one budget");
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+
+// Tiled copies with four coordinates (column, factor, row, expert).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int c0,
+                                            int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(desc)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const void* desc, uint32_t src, int c0, int c1, int c2,
+                                             int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+      :
+      : "l"(reinterpret_cast<uint64_t>(desc)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+struct GatedParams {
+  const float* bias;  // forward: (E, 2, M) or NULL
+  float* sums;        // backward: (E, row blocks of 32, 2, M) partial column sums or NULL
+  int rows, k, m, batch;
+  int act;            // 0 GELU (tanh form), 1 SiLU
+  int save;           // forward: write a and s
+};
+
+// act(g) and act'(g) through one sigmoid: act = g sigma(w), act' = sigma (1 + g (1 - sigma) w').
+// GELU's tanh form is w = 2 sqrt(2/pi) (g + 0.044715 g^3), SiLU is w = g.
+__device__ __forceinline__ void gate_and_slope(float g, int act, float& a, float& slope) {
+  constexpr float K0 = 1.5957691216057308f, K1 = K0 * 0.044715f, L = 1.4426950408889634f;
+  float w, dw;
+  if (act == 0) {
+    const float g2 = g * g;
+    w = g * fmaf(g2, K1, K0);
+    dw = fmaf(g2, 3.0f * K1, K0);
+  } else {
+    w = g;
+    dw = 1.0f;
+  }
+  float e, sg;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-L * w));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.0f + e));
+  a = g * sg;
+  slope = sg * fmaf(g * (1.0f - sg), dw, 1.0f);
+}
+
+// MODE 0: forward. A = x (rows x k), B = w_in as (k, m, 2 E), both K-major.
+// MODE 1: backward. A = dy (rows x k, K-major), B = w_out (m contiguous: MN-major).
+template <bool PAIR, int MODE>
+__global__ void __launch_bounds__(THREADS, 1)
+gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+             const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_s,
+             const __grid_constant__ CUtensorMap map_d, const GatedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  constexpr int NSTAGE = PAIR ? STAGES_PAIR : STAGES;
+  constexpr int BSTAGE = PAIR ? B_BYTES / 2 : B_BYTES;
+  constexpr int TM = PAIR ? 2 * BM : BM;
+  constexpr int TN = MODE == 0 ? HALF : BN;  // hidden units per tile
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + NSTAGE * A_BYTES;
+  uint8_t* sEpi = smem + PIPE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + EPI_WARPS * EPI_TILES * TILE_BYTES);
+  // full[NSTAGE], empty[NSTAGE], accumulator full[2], accumulator empty[2], epilogue input[8]
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = smem_u32(bars + NSTAGE);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * NSTAGE);
+  const uint32_t bar_tempty = smem_u32(bars + 2 * NSTAGE + 2);
+  const uint32_t bar_in = smem_u32(bars + 2 * NSTAGE + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NSTAGE + 4 + EPI_WARPS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const int cta = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int ncta = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < NSTAGE; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_tfull + 8 * s, 1);
+      mbar_init(bar_tempty + 8 * s, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+    }
+    for (int s = 0; s < EPI_WARPS; ++s) mbar_init(bar_in + 8 * s, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // the peer's barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_m = (p.rows + TM - 1) / TM;
+  const int num_n = (p.m + TN - 1) / TN;
+  const int k_tiles = (p.k + BK - 1) / BK;
+  const int num_tiles = p.batch * num_m * num_n;
+  // Hidden units fastest, then rows, then experts: CTAs that run together share rows of A.
+  auto decode = [&](int tile, int& b, int& mt, int& nt) {
+    nt = tile % num_n;
+    tile /= num_n;
+    mt = tile % num_m;
+    b = tile / num_m;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full_base = PAIR ? mapa_shared(bar_full, 0) : bar_full;
+      for (int tile = cta; tile < num_tiles && ok; tile += ncta) {
+        int b, mt, nt;
+        decode(tile, b, mt, nt);
+        const int m0 = mt * TM + static_cast<int>(rank) * BM;
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, nullptr, 0)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = full_base + 8 * stage;
+          if (!PAIR) {
+            mbar_expect_tx(full, A_BYTES + BSTAGE);
+          } else if (rank == 0) {
+            mbar_expect_tx(bar_full + 8 * stage, 2 * (A_BYTES + BSTAGE));
+          }
+          const uint32_t a_dst = smem_u32(sA + stage * A_BYTES);
+          const uint32_t b_dst = smem_u32(sB + stage * BSTAGE);
+          const int k0 = kt * BK;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+            if (PAIR) {
+              tma_load_3d_pair(dst, map, full, c0, c1, c2);
+            } else {
+              tma_load_3d(dst, map, full, c0, c1, c2);
+            }
+          };
+          load(a_dst, &map_a, k0, m0, b);
+          if (MODE == 0) {
+            if (PAIR) {
+              load(b_dst, &map_b, k0, nt * TN, 2 * b + static_cast<int>(rank));
+            } else {
+              load(b_dst, &map_b, k0, nt * TN, 2 * b);
+              load(b_dst + B_BYTES / 2, &map_b, k0, nt * TN, 2 * b + 1);
+            }
+          } else {
+            const int n0 = nt * TN + static_cast<int>(rank) * HALF;
+#pragma unroll
+            for (int j = 0; j < (PAIR ? HALF : BN) / 64; ++j)
+              load(b_dst + j * CHUNK_BYTES, &map_b, n0 + 64 * j, k0, b);
+          }
+          if (++stage == NSTAGE) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {  // copies in flight get a bounded chance to land before the CTA exits
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) __nanosleep(256);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = umma_idesc_bf16(TM, BN, 0, MODE);
+      const uint32_t b_lbo = MODE ? CHUNK_BYTES : 16, b_step = MODE ? 2048 : 32;
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int tile = cta; tile < num_tiles && ok; tile += ncta, ++local) {
+        const int slot = local & 1;
+        const uint32_t use = static_cast<uint32_t>(local >> 1);
+        if (!mbar_wait(bar_tempty + 8 * slot, (use & 1) ^ 1, abort_flag, nullptr, 0)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + slot * BN;
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, nullptr, 0)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(sA + stage * A_BYTES);
+          const uint32_t b_addr = smem_u32(sB + stage * BSTAGE);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            const uint64_t adesc = umma_smem_desc(a_addr + k * 32, 16, 1024);
+            const uint64_t bdesc = umma_smem_desc(b_addr + k * b_step, b_lbo, 1024);
+            if (PAIR) {
+              umma_bf16_pair(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+            } else {
+              umma_bf16(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+            }
+          }
+          if (PAIR) {
+            umma_commit_pair(bar_empty + 8 * stage, 3);
+          } else {
+            umma_commit(bar_empty + 8 * stage);
+          }
+          if (++stage == NSTAGE) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (PAIR) {
+          umma_commit_pair(bar_tfull + 8 * slot, 3);
+        } else {
+          umma_commit(bar_tfull + 8 * slot);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int ew = warp - 2;
+    const int quad = warp & 3;   // TMEM lanes this warp may read
+    const int half = ew >> 2;
+    uint8_t* tiles = sEpi + ew * EPI_TILES * TILE_BYTES;
+    const uint32_t st_row = static_cast<uint32_t>(lane) * 64u;
+    const uint32_t st_xor = (static_cast<uint32_t>(lane) >> 1) & 3u;
+    constexpr int CHUNKS = TN / 32 / 2;  // 32-column chunks per warp and tile
+    const uint32_t in_bar = bar_in + 8 * ew;
+    const uint32_t tempty_base = PAIR ? mapa_shared(bar_tempty, 0) : bar_tempty;
+    uint32_t in_phase = 0;
+    int local = 0;
+    bool ok = true;
+    // One row of a chunk (32 packed values) into a staging tile.
+    auto stage_row = [&](uint8_t* tile, const uint32_t (&w)[16]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(tile + st_row + ((static_cast<uint32_t>(i) ^ st_xor) << 4)) =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    };
+    for (int tile = cta; tile < num_tiles && ok; tile += ncta, ++local) {
+      int b, mt, nt;
+      decode(tile, b, mt, nt);
+      const int slot = local & 1;
+      const uint32_t use = static_cast<uint32_t>(local >> 1);
+      const int row0 = mt * TM + static_cast<int>(rank) * BM + quad * 32;
+      const int n0 = nt * TN;
+      // Backward: the saved factors of a chunk (tiles 2 and 3), fetched ahead.
+      auto fetch = [&](int col0) {
+        if (lane == 0) {
+          mbar_expect_tx(in_bar, 2 * TILE_BYTES);
+          tma_load_4d(smem_u32(tiles + 2 * TILE_BYTES), &map_s, in_bar, col0, 0, row0, b);
+          tma_load_4d(smem_u32(tiles + 3 * TILE_BYTES), &map_s, in_bar, col0, 1, row0, b);
+        }
+      };
+      if (MODE == 1 && n0 + half * CHUNKS * 32 < p.m) fetch(n0 + half * CHUNKS * 32);
+      const bool got = mbar_wait(bar_tfull + 8 * slot, use & 1, abort_flag, nullptr, 0);
+      if (!__all_sync(0xffffffffu, got)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = half * CHUNKS; c < half * CHUNKS + CHUNKS; ++c) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= p.m) break;
+        const uint32_t acc =
+            tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + slot * BN + c * 32;
+        if (MODE == 0) {
+          uint32_t rg[32], ru[32];
+          tmem_ld_32x32(acc, rg);
+          tmem_ld_32x32(acc + HALF, ru);
+          tmem_ld_wait();
+          if (p.bias) {
+            const float* bg = p.bias + (2ll * b) * p.m + col0;
+            const float* bu = bg + p.m;
+            if (col0 + 32 <= p.m) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 g4 = __ldg(reinterpret_cast<const float4*>(bg) + i);
+                const float4 u4 = __ldg(reinterpret_cast<const float4*>(bu) + i);
+                rg[4 * i] = __float_as_uint(__uint_as_float(rg[4 * i]) + g4.x);
+                rg[4 * i + 1] = __float_as_uint(__uint_as_float(rg[4 * i + 1]) + g4.y);
+                rg[4 * i + 2] = __float_as_uint(__uint_as_float(rg[4 * i + 2]) + g4.z);
+                rg[4 * i + 3] = __float_as_uint(__uint_as_float(rg[4 * i + 3]) + g4.w);
+                ru[4 * i] = __float_as_uint(__uint_as_float(ru[4 * i]) + u4.x);
+                ru[4 * i + 1] = __float_as_uint(__uint_as_float(ru[4 * i + 1]) + u4.y);
+                ru[4 * i + 2] = __float_as_uint(__uint_as_float(ru[4 * i + 2]) + u4.z);
+                ru[4 * i + 3] = __float_as_uint(__uint_as_float(ru[4 * i + 3]) + u4.w);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col0 + i < p.m) {
+                  rg[i] = __float_as_uint(__uint_as_float(rg[i]) + __ldg(bg + i));
+                  ru[i] = __float_as_uint(__uint_as_float(ru[i]) + __ldg(bu + i));
+                }
+            }
+          }
+          uint32_t wh[16], wa[16], ws[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a0, a1, s0, s1;
+            const float u0 = __uint_as_float(ru[2 * i]), u1 = __uint_as_float(ru[2 * i + 1]);
+            gate_and_slope(__uint_as_float(rg[2 * i]), p.act, a0, s0);
+            gate_and_slope(__uint_as_float(rg[2 * i + 1]), p.act, a1, s1);
+            wh[i] = pack_bf16x2(a0 * u0, a1 * u1);
+            wa[i] = pack_bf16x2(a0, a1);
+            ws[i] = pack_bf16x2(s0 * u0, s1 * u1);
+          }
+          // The staging tiles are free once the TMA engine has read their last contents.
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          stage_row(tiles, wh);
+          if (p.save) {
+            stage_row(tiles + TILE_BYTES, ws);
+            stage_row(tiles + 2 * TILE_BYTES, wa);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&map_h, smem_u32(tiles), col0, row0, b);
+            if (p.save) {
+              tma_store_4d(&map_s, smem_u32(tiles + TILE_BYTES), col0, 0, row0, b);
+              tma_store_4d(&map_s, smem_u32(tiles + 2 * TILE_BYTES), col0, 1, row0, b);
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          uint32_t r[32];
+          tmem_ld_32x32(acc, r);
+          const bool in = mbar_wait(in_bar, in_phase, abort_flag, nullptr, 0);
+          in_phase ^= 1;
+          if (!__all_sync(0xffffffffu, in)) {
+            ok = false;
+            break;
+          }
+          uint4 qs[4], qa[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t off = st_row + ((static_cast<uint32_t>(i) ^ st_xor) << 4);
+            qs[i] = *reinterpret_cast<const uint4*>(tiles + 2 * TILE_BYTES + off);
+            qa[i] = *reinterpret_cast<const uint4*>(tiles + 3 * TILE_BYTES + off);
+          }
+          tmem_ld_wait();
+          __syncwarp();
+          if (c + 1 < half * CHUNKS + CHUNKS && col0 + 32 < p.m) fetch(col0 + 32);
+          uint32_t wg[16], wu[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint4 s4 = qs[i >> 2], a4 = qa[i >> 2];
+            const uint32_t sw = (i & 3) == 0 ? s4.x : (i & 3) == 1 ? s4.y : (i & 3) == 2 ? s4.z : s4.w;
+            const uint32_t aw = (i & 3) == 0 ? a4.x : (i & 3) == 1 ? a4.y : (i & 3) == 2 ? a4.z : a4.w;
+            const float2 fs = unpack_bf16x2(sw), fa = unpack_bf16x2(aw);
+            const float d0 = __uint_as_float(r[2 * i]), d1 = __uint_as_float(r[2 * i + 1]);
+            wg[i] = pack_bf16x2(d0 * fs.x, d1 * fs.y);
+            wu[i] = pack_bf16x2(d0 * fa.x, d1 * fa.y);
+          }
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          stage_row(tiles, wg);
+          stage_row(tiles + TILE_BYTES, wu);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_4d(&map_d, smem_u32(tiles), col0, 0, row0, b);
+            tma_store_4d(&map_d, smem_u32(tiles + TILE_BYTES), col0, 1, row0, b);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          if (p.sums && row0 < p.rows) {
+            // Column sums of the 32 staged rows: lanes 0-15 take the even rows, 16-31 the odd ones
+            // of two columns each (rows past the end hold zeros). Written, not added: a second
+            // kernel joins the row blocks in a fixed order.
+            const long long blocks = (p.rows + 31) / 32;
+            const uint32_t pair = lane & 15, odd = lane >> 4;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint32_t rr = 2 * i + odd;
+                const uint32_t off = rr * 64u + (((pair >> 2) ^ ((rr >> 1) & 3u)) << 4) + (pair & 3) * 4u;
+                const float2 f = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(tiles + w * TILE_BYTES + off));
+                s0 += f.x;
+                s1 += f.y;
+              }
+              s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
+              s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
+              const int col = col0 + 2 * static_cast<int>(pair);
+              if (odd == 0 && col < p.m)
+                *reinterpret_cast<float2*>(p.sums + ((b * blocks + row0 / 32) * 2 + w) * p.m + col) =
+                    make_float2(s0, s1);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) {
+          mbar_arrive_cluster(tempty_base + 8 * slot);
+        } else {
+          mbar_arrive(bar_tempty + 8 * slot);
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (!ok) {  // an input tile may still be in flight
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000) __nanosleep(256);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // neither CTA leaves while its peer can touch its barriers or TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    if (PAIR) {
+      tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    } else {
+      tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+  }
+}
+
+// out[e][c] (+)= sum over the row blocks of sums[e][block][c], blocks in order within a thread
+// group and groups in order, so the result does not depend on scheduling.
+__global__ void __launch_bounds__(256)
+gated_join_sums_kernel(const float* __restrict__ sums, float* __restrict__ out, int blocks, int cols,
+                       int accumulate) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  const float* src = sums + static_cast<long long>(blockIdx.y) * blocks * cols;
+  float s = 0.0f;
+  if (c < cols)
+    for (int i = group; i < blocks; i += 8) s += src[static_cast<long long>(i) * cols + c];
+  part[group][lane] = s;
+  __syncthreads();
+  if (group == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) s += part[i][lane];
+    float* dst = out + static_cast<long long>(blockIdx.y) * cols + c;
+    *dst = accumulate ? *dst + s : s;
+  }
+}
+
+int fail(const char* what, int code = -1) {
+  set_error("%s (code %d)", what, code);
+  return code;
+}
+
+// (e, rows, 2, m) contiguous bf16 as a 4-D tensor with 32 x 32 boxes.
+int make_pair_map(CUtensorMap* map, const void* ptr, uint64_t m, uint64_t rows, uint64_t e) {
+  cuuint64_t dims[4] = {m, 2, rows, e};
+  cuuint64_t strides[3] = {m * 2, m * 4, rows * m * 4};
+  cuuint32_t box[4] = {32, 1, 32, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = tma_encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
+                                strides, box, estr, CU_TENSOR_MAP_SWIZZLE_64B);
+  return r == CUDA_SUCCESS ? 0 : fail("cuTensorMapEncodeTiled failed", -3);
+}
+
+struct DeviceInfo {
+  int sms, pairs;
+};
+
+// Per-device set-up (shared-memory limits, resident CTA pairs), done once per device.
+int device_info(DeviceInfo* out) {
+  constexpr int MAX_DEVICES = 64;
+  static DeviceInfo known[MAX_DEVICES];
+  static bool ready[MAX_DEVICES];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev >= MAX_DEVICES) return fail("no current device", -4);
+  if (!ready[dev]) {
+    DeviceInfo d = {0, 0};
+    e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+    const void* kernels[4] = {reinterpret_cast<const void*>(gated_kernel<false, 0>),
+                              reinterpret_cast<const void*>(gated_kernel<false, 1>),
+                              reinterpret_cast<const void*>(gated_kernel<true, 0>),
+                              reinterpret_cast<const void*>(gated_kernel<true, 1>)};
+    for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+      e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) {
+      set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+      return -4;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr;
+    memset(&attr, 0, sizeof(attr));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(d.sms & ~1));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&d.pairs, gated_kernel<true, 0>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      d.pairs = 0;
+    }
+    known[dev] = d;
+    ready[dev] = true;
+  }
+  *out = known[dev];
+  return 0;
+}
+
+template <int MODE>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh, const CUtensorMap& ms,
+           const CUtensorMap& md, const GatedParams& p, const DeviceInfo& info, bool pair,
+           cudaStream_t stream) {
+  const int tm = pair ? 2 * BM : BM, tn = MODE == 0 ? HALF : BN;
+  const long long tiles =
+      static_cast<long long>(p.batch) * ((p.rows + tm - 1) / tm) * ((p.m + tn - 1) / tn);
+  if (tiles > 0x7fffffff) return fail("gated mlp: too many tiles");
+  const long long most = pair ? info.pairs : info.sms;
+  const unsigned units = static_cast<unsigned>(tiles < most ? tiles : most);
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(pair ? 2 * units : units);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = pair ? 1 : 0;
+  const cudaError_t e =
+      pair ? cudaLaunchKernelEx(&cfg, gated_kernel<true, MODE>, ma, mb, mh, ms, md, p)
+           : cudaLaunchKernelEx(&cfg, gated_kernel<false, MODE>, ma, mb, mh, ms, md, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+    return -5;
+  }
+  return 0;
+}
+
+int check_args(const VmoeGatedArgs* a) {
+  if (a->e < 0 || a->rows < 0 || a->k < 1 || a->m < 1) return fail("gated mlp: bad sizes");
+  if (a->rows > (1 << 28) || a->k > (1 << 24) || a->m > (1 << 24) || a->e > (1 << 20))
+    return fail("gated mlp: sizes out of range");
+  if (a->k % 8 || a->m % 8 || a->lda % 8 || a->a_batch_stride % 8)
+    return fail("gated mlp: widths and strides must be multiples of 8 elements");
+  const void* ptrs[6] = {a->a, a->w, a->hid, a->saved, a->grad, a->bias};
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return fail("gated mlp: operands must be 16-byte aligned");
+  if (a->act != 0 && a->act != 1) return fail("gated mlp: unknown activation");
+  return 0;
+}
+
+bool use_pairs(const VmoeGatedArgs* a, const DeviceInfo& info, int tn) {
+  // Pairs pay off once there is a 256-row tile for at least every other pair of SMs.
+  const long long tiles = a->e * ((a->rows + 2 * BM - 1) / (2 * BM)) * ((a->m + tn - 1) / tn);
+  return info.pairs > 0 && a->rows >= 2 * BM && tiles >= info.pairs / 2;
+}
+
+}  // namespace
+}  // namespace vmoe
+
+using namespace vmoe;
+
+extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc = check_args(a);
+  if (rc) return rc;
+  if (a->e == 0 || a->rows == 0) return 0;
+  DeviceInfo info;
+  if ((rc = device_info(&info))) return rc;
+  CUtensorMap ma, mb, mh, ms;
+  memset(&ms, 0, sizeof(ms));
+  if ((rc = make_bf16_map(&ma, a->a, a->k, a->rows, a->e, a->lda, a->a_batch_stride, BM, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_bf16_map(&mb, a->w, a->k, a->m, 2 * a->e, a->k, a->m * a->k, HALF, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_bf16_map(&mh, a->hid, a->m, a->rows, a->e, a->m, a->rows * a->m, 32, 32,
+                          CU_TENSOR_MAP_SWIZZLE_64B)))
+    return rc;
+  if (a->saved && (rc = make_pair_map(&ms, a->saved, a->m, a->rows, a->e))) return rc;
+  GatedParams p;
+  memset(&p, 0, sizeof(p));
+  p.bias = a->bias;
+  p.rows = static_cast<int>(a->rows);
+  p.k = static_cast<int>(a->k);
+  p.m = static_cast<int>(a->m);
+  p.batch = static_cast<int>(a->e);
+  p.act = a->act;
+  p.save = a->saved != nullptr;
+  return launch<0>(ma, mb, mh, ms, ms, p, info, use_pairs(a, info, HALF), stream);
+}
+
+extern "C" int64_t vmoe_gated_bwd_sums_bytes(int64_t e, int64_t rows, int64_t m) {
+  return e * ((rows + 31) / 32) * 2 * m * 4;
+}
+
+extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, float* sums, float* db, int32_t accumulate,
+                              vmoe_stream_t stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc = check_args(a);
+  if (rc) return rc;
+  if (a->e == 0 || a->rows == 0) return 0;
+  if ((sums == nullptr) != (db == nullptr)) return fail("gated mlp: bias gradient needs scratch");
+  if (reinterpret_cast<uintptr_t>(sums) & 15) return fail("gated mlp: scratch must be 16-byte aligned");
+  DeviceInfo info;
+  if ((rc = device_info(&info))) return rc;
+  const bool pair = use_pairs(a, info, BN);
+  CUtensorMap ma, mb, ms, md;
+  if ((rc = make_bf16_map(&ma, a->a, a->k, a->rows, a->e, a->lda, a->a_batch_stride, BM, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_bf16_map(&mb, a->w, a->m, a->k, a->e, a->m, a->m * a->k, BK, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_pair_map(&ms, a->saved, a->m, a->rows, a->e))) return rc;
+  if ((rc = make_pair_map(&md, a->grad, a->m, a->rows, a->e))) return rc;
+  GatedParams p;
+  memset(&p, 0, sizeof(p));
+  p.sums = sums;
+  p.rows = static_cast<int>(a->rows);
+  p.k = static_cast<int>(a->k);
+  p.m = static_cast<int>(a->m);
+  p.batch = static_cast<int>(a->e);
+  if ((rc = launch<1>(ma, mb, ms, ms, md, p, info, pair, stream))) return rc;
+  if (sums) {
+    const int blocks = static_cast<int>((a->rows + 31) / 32), cols = static_cast<int>(2 * a->m);
+    if (a->e > 65535) return fail("gated mlp: too many experts");
+    gated_join_sums_kernel<<<dim3((cols + 31) / 32, static_cast<unsigned>(a->e)), 256, 0, stream>>>(
+        sums, db, blocks, cols, accumulate);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+      set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+      return -5;
+    }
+  }
+  return 0;
+}

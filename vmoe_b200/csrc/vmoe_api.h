@@ -78,6 +78,31 @@ typedef struct VmoeGemmArgs {
 
 VMOE_API int vmoe_gemm_bf16(const VmoeGemmArgs* args, vmoe_stream_t stream);
 
+// ----------------------------------------------------------------------------- gated MLP
+// Forward: hid (e, rows, m) = act(g) * u with g = A Wg^T + bias[0], u = A Wu^T + bias[1] per expert;
+// A (e, rows, k) bf16 with row stride lda, w (e, 2, m, k) bf16 (gate, up), bias (e, 2, m) fp32 or NULL.
+// With `saved` (e, rows, 2, m) bf16, it receives u act'(g) and act(g) for the backward pass.
+// Backward: A = dy (e, rows, k), w = w_out (e, k, m); grad (e, rows, 2, m) = (dh * saved[0],
+// dh * saved[1]) with dh = dy w, i.e. the gradients of g and u. With `sums` (scratch of
+// vmoe_gated_bwd_sums_bytes) and db (e, 2, m) fp32, db receives (accumulate: is increased by) their
+// column sums, added up in an order that does not depend on scheduling.
+// k, m, lda and a_batch_stride are multiples of 8, pointers 16-byte aligned, everything but A contiguous.
+typedef struct VmoeGatedArgs {
+  const void* a;
+  const void* w;
+  const float* bias;
+  void* hid;
+  void* saved;
+  void* grad;
+  int64_t e, rows, k, m;
+  int64_t lda, a_batch_stride;
+  int32_t act;  // 0 GELU (tanh form), 1 SiLU
+} VmoeGatedArgs;
+VMOE_API int vmoe_gated_fwd(const VmoeGatedArgs* args, vmoe_stream_t stream);
+VMOE_API int64_t vmoe_gated_bwd_sums_bytes(int64_t e, int64_t rows, int64_t m);
+VMOE_API int vmoe_gated_bwd(const VmoeGatedArgs* args, float* sums, float* db, int32_t accumulate,
+                            vmoe_stream_t stream);
+
 // ----------------------------------------------------------------------------- elementwise
 // LayerNorm over the last dim of bf16 x[rows][h] (h % 8 == 0, h <= 2048); gamma/beta fp32 or
 // NULL; mean/rstd (fp32 per row) are saved for the backward pass when non-NULL.

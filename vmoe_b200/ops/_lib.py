@@ -80,6 +80,17 @@ class PushArgs(ctypes.Structure):
   ]
 
 
+class GatedArgs(ctypes.Structure):
+  """Mirror of ``VmoeGatedArgs``."""
+  _fields_ = [
+      ("a", ctypes.c_void_p), ("w", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+      ("hid", ctypes.c_void_p), ("saved", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+      ("e", ctypes.c_int64), ("rows", ctypes.c_int64), ("k", ctypes.c_int64),
+      ("m", ctypes.c_int64), ("lda", ctypes.c_int64), ("a_batch_stride", ctypes.c_int64),
+      ("act", ctypes.c_int32),
+  ]
+
+
 class DistillArgs(ctypes.Structure):
   """Mirror of ``VmoeDistillArgs``."""
   _fields_ = [
@@ -112,6 +123,7 @@ def lib() -> ctypes.CDLL:
       l.vmoe_last_error.restype = ctypes.c_char_p
       l.vmoe_top_logits_max_classes.restype = ctypes.c_int64
       l.vmoe_distill_max_classes.restype = ctypes.c_int64
+      l.vmoe_gated_bwd_sums_bytes.restype = ctypes.c_int64
       _lib = l
   return _lib
 
