@@ -2,16 +2,20 @@
 // with the log-sum-exp of all the others, and the divergence of a student from such a teacher
 // with its gradient. Logits are bf16, fp16 or fp32 rows of any stride and alignment.
 //
-// Every kernel gives a row to one CTA, or to a cluster of 2, 4 or 8 CTAs that share it when there
-// are few rows (each takes a range of columns, results meet in distributed shared memory), reads
-// it in 16-byte vectors from the first aligned address on and the at most 14 edge elements one by
-// one.
+// The two kernels that reduce a row bring it to shared memory first: one bulk asynchronous copy of
+// its whole 16-byte vectors, which needs no registers and has the whole row in flight at once; the
+// at most two partial vectors at the ends are filled element by element, padded with -inf. A
+// second pass over the row then costs no memory traffic. A row belongs to one CTA, or to a
+// cluster of 2, 4 or 8 CTAs when there are few rows or the row does not fit one (each takes a range
+// of vectors, results meet in distributed shared memory).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "ptx_sm100.cuh"
 #include "vmoe_api.h"
@@ -22,8 +26,6 @@ void set_error(const char* fmt, const char* a, int code);
 
 namespace {
 
-constexpr int DT = 256;  // threads per CTA of the kernels in this file
-constexpr int DW = DT / 32;
 constexpr int MAX_PARTS = 8;  // CTAs that can share a row (portable cluster size)
 
 typedef unsigned long long u64;
@@ -92,17 +94,97 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// Order of the values as unsigned integers: -inf < ... < -0 = +0 < ... < +inf < NaN; 0 is below
-// every value and stands for "nothing here".
-__device__ __forceinline__ uint32_t key_of(float v) {
-  const uint32_t b = __float_as_uint(v);
-  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  if ((b & 0x7fffffffu) == 0) return 0x80000000u;
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+// Order of the values as unsigned integers (16 bits of them for 16-bit types): -inf < ... < -0 = +0
+// < ... < +inf < NaN; 0 is below every value and stands for "nothing here".
+template <typename T>
+struct Order;
+template <>
+struct Order<float> {
+  static __device__ __forceinline__ uint32_t key(uint32_t b) {
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    if ((b & 0x7fffffffu) == 0) return 0x80000000u;
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  }
+  static __device__ __forceinline__ float value(uint32_t key) {
+    if (key == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+    return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+  }
+  // Largest of a vector joined with `m`; NaN wins.
+  static __device__ __forceinline__ uint32_t largest(uint32_t m, const uint4& q) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float f = __uint_as_float(m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(f) : "f"(__uint_as_float(w[i])));
+    return __float_as_uint(f);
+  }
+  static constexpr uint32_t kLow = 0xff800000u;  // -inf, as `largest` starts
+  static __device__ __forceinline__ uint32_t key_of_largest(uint32_t m) { return key(m); }
+  static __device__ __forceinline__ bool all_below(uint32_t m, float bound) {
+    return __uint_as_float(m) < bound;
+  }
+};
+template <typename T>
+struct Order16 {
+  static constexpr uint32_t kInf = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  static __device__ __forceinline__ uint32_t key(uint32_t b) {
+    if ((b & 0x7fffu) > kInf) return 0xffffu;
+    if ((b & 0x7fffu) == 0) return 0x8000u;
+    return b ^ ((b >> 15) ? 0xffffu : 0x8000u);
+  }
+  static __device__ __forceinline__ float value(uint32_t key) {
+    const uint32_t b = key == 0xffffu ? 0x7fffu : key ^ ((key >> 15) ? 0x8000u : 0xffffu);
+    const unsigned short h = static_cast<unsigned short>(b);
+    return to_float(*reinterpret_cast<const T*>(&h));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (std::is_same<T, __half>::value) {
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    } else {
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    }
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t largest(uint32_t m, const uint4& q) {
+    return max2(m, max2(max2(q.x, q.y), max2(q.z, q.w)));
+  }
+  static constexpr uint32_t kLow = 0x80008000u | kInf | (kInf << 16);
+  static __device__ __forceinline__ uint32_t key_of_largest(uint32_t m) {
+    const uint32_t a = key(m & 0xffffu), b = key(m >> 16);
+    return a > b ? a : b;
+  }
+  static __device__ __forceinline__ bool all_below(uint32_t m, float bound) {
+    const unsigned short h0 = static_cast<unsigned short>(m), h1 = static_cast<unsigned short>(m >> 16);
+    return to_float(*reinterpret_cast<const T*>(&h0)) < bound &&
+           to_float(*reinterpret_cast<const T*>(&h1)) < bound;
+  }
+};
+template <>
+struct Order<__nv_bfloat16> : Order16<__nv_bfloat16> {};
+template <>
+struct Order<__half> : Order16<__half> {};
+
+// Bits of element e of a vector.
+template <typename T>
+__device__ __forceinline__ uint32_t bits_at(const uint4& q, int e) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if (sizeof(T) == 4) return w[e];
+  return e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
 }
-__device__ __forceinline__ float value_of(uint32_t key) {
-  if (key == 0xffffffffu) return __uint_as_float(0x7fffffffu);
-  return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+
+// Sum of 2^(x c + a) over a vector.
+template <typename T>
+__device__ __forceinline__ void add_exponentials(const uint4& q, float c, float a, f32x2& sum) {
+  constexpr int W = Vec<T>::W;
+  float v[W];
+  unpack(q, v, T());
+  const f32x2 cc = f2_pack(c, c), aa = f2_pack(a, a);
+#pragma unroll
+  for (int e = 0; e < W; e += 2) {
+    float t0, t1;
+    f2_unpack(f2_fma(f2_pack(v[e], v[e + 1]), cc, aa), t0, t1);
+    sum = f2_add(sum, f2_pack(exp2_approx(t0), exp2_approx(t1)));
+  }
 }
 
 // Values beyond this are not multiplied by log2(e) / temperature before the row's anchor is taken
@@ -123,7 +205,7 @@ struct RowLayout {
   }
 };
 
-template <typename V, typename Op>
+template <int DT, typename V, typename Op>
 __device__ __forceinline__ V block_reduce(V v, V* red, Op op) {  // result in every thread
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
@@ -133,7 +215,7 @@ __device__ __forceinline__ V block_reduce(V v, V* red, Op op) {  // result in ev
   __syncthreads();
   V t = red[0];
 #pragma unroll
-  for (int i = 1; i < DW; ++i) t = op(t, red[i]);
+  for (int i = 1; i < DT / 32; ++i) t = op(t, red[i]);
   return t;
 }
 struct Sum {
@@ -148,77 +230,111 @@ struct Min {
   __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
 };
 
+// The vectors v0 .. v1 - 1 of a row that belong to this CTA, on their way to shared memory. Vector j
+// holds the elements j W - off .. j W - off + W - 1 (off: the row's place within 16 bytes).
+template <typename T, int DT>
+struct StagedRow {
+  static constexpr int W = Vec<T>::W;
+  int n, off, vectors, v0, v1;
+  const uint4* row;  // [v1 - v0] in shared memory
+
+  __device__ __forceinline__ StagedRow(const T* x, int n_, int part, int parts, uint4* smem, uint32_t bar)
+      : n(n_), row(smem) {
+    off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    vectors = (off + n + W - 1) / W;
+    const int per = (vectors + parts - 1) / parts;
+    v0 = min(part * per, vectors);
+    v1 = min(v0 + per, vectors);
+    const int b0 = v0 + (v0 == 0 && off > 0 ? 1 : 0);
+    const int b1 = v1 - (v1 == vectors && (off + n) % W ? 1 : 0);
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+      mbar_init(bar, 1);
+      fence_mbar_init();
+      const uint32_t bytes = b1 > b0 ? static_cast<uint32_t>(b1 - b0) * 16u : 0u;
+      mbar_expect_tx(bar, bytes);
+      if (bytes)
+        asm volatile(
+            "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+            :
+            : "r"(smem_u32(smem + (b0 - v0))), "l"(x - off + static_cast<long long>(b0) * W), "r"(bytes),
+              "r"(bar)
+            : "memory");
+    }
+    // Partial vectors at the row's ends (one vector may be both).
+    const int e = tid % W;
+    const int j = tid < W ? 0 : vectors - 1;
+    if (tid < 2 * W && j >= v0 && j < v1 && (j < b0 || j >= b1)) {
+      const int at = j * W + e - off;
+      reinterpret_cast<T*>(smem + (j - v0))[e] =
+          at >= 0 && at < n ? x[at] : from_float<T>(-INFINITY);
+    }
+  }
+  __device__ __forceinline__ int elements() const {  // real elements of this part
+    return v1 > v0 ? min(n, v1 * W - off) - max(0, v0 * W - off) : 0;
+  }
+  __device__ __forceinline__ int position(int i, int e) const { return (v0 + i) * W + e - off; }
+};
+
 // ------------------------------------------------------------------------------- top logits
-constexpr int TOP_CAP = 2048;  // candidates that shared memory holds
+constexpr int TOP_CAP = 1024;  // candidates that shared memory holds
 constexpr int TOP_K_MAX = 256;
 
-// One part of a row: NV vectors per thread stay in registers. The k largest of the threads'
-// maxima (found by bisection on their order keys with one block-wide count per step) bound the
-// k-th largest value from below, so everything not below that bound is a candidate: about k of
-// them for values in no particular order. Candidates are ranked by counting larger ones. Ties
-// that would overflow the candidate list (a row of equal values) take an exact bisection over
-// values and then positions instead. The same pass sums the exponentials of everything that is
-// not a candidate, relative to the bound; candidates that lose and a sum that underflows get
-// anchors of their own, so that `rest` is right however far below the kept values it lies.
-template <typename T, int NV>
+// The k largest of the threads' maxima (found by bisection on their order keys, one block-wide count
+// per step) bound the k-th largest value from below, so everything not below that bound is a
+// candidate: somewhat more than k of them for values in no particular order. Where there are too
+// many (more kept than threads, rows of equal values) the bisection goes on over all values, and
+// over positions among equal ones. Candidates are ranked by counting the larger ones. The pass that
+// collects them also sums the exponentials of everything else relative to the bound; candidates
+// that lose and a sum that underflows get anchors of their own, so that `rest` is right however far
+// below the kept values it lies. All sums have a fixed order.
+template <typename T, int DT>
 __global__ void __launch_bounds__(DT)
 top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, float c, double inv_t,
                   int parts, T* __restrict__ values, int* __restrict__ indices,
                   float* __restrict__ rest) {
   constexpr int W = Vec<T>::W;
-  __shared__ u64 cand[TOP_CAP];
-  __shared__ u64 top[TOP_K_MAX];
-  __shared__ uint32_t red_u[DW];
-  __shared__ float red_f[DW];
-  __shared__ int count;
+  using Ord = Order<T>;
+  extern __shared__ __align__(16) uint4 row_smem[];
+  __shared__ __align__(16) u64 cand[TOP_CAP];
+  __shared__ __align__(16) u64 sorted[TOP_CAP];
+  __shared__ uint32_t red_u[DT / 32];
+  __shared__ float red_f[DT / 32];
   __shared__ float2 part_rest[MAX_PARTS];
+  __shared__ __align__(8) uint64_t bar_mem;
+  __shared__ int count, gave_up;
   const int tid = threadIdx.x;
   const int part = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long r = blockIdx.x / parts;
   const T* x = logits + r * ld;
-  const RowLayout<T> lay(x, n);
-  const int per = (lay.vectors + parts - 1) / parts;
-  const int v0 = min(part * per, lay.vectors), v1 = min(v0 + per, lay.vectors);
-  const uint4* xv = reinterpret_cast<const uint4*>(x + lay.head);
+  const uint32_t bar = smem_u32(&bar_mem);
+  const StagedRow<T, DT> st(x, n, part, parts, row_smem, bar);
+  const int nv = st.v1 - st.v0;
+  const int mine = min(k, st.elements());  // entries this part can contribute
+  if (tid == 0) count = gave_up = 0;
+  __syncthreads();
+  if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
 
-  // This part's elements: up to NV vectors per thread, and one edge element in part 0.
-  uint4 raw[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int j = v0 + tid + i * DT;
-    if (j < v1) raw[i] = __ldg(xv + j);
+  uint32_t m0 = Ord::kLow, m1 = Ord::kLow;
+  int i = tid;
+  for (; i + DT < nv; i += 2 * DT) {
+    m0 = Ord::largest(m0, st.row[i]);
+    m1 = Ord::largest(m1, st.row[i + DT]);
   }
-  const int edges = part == 0 ? lay.head + lay.tail : 0;
-  const bool has_edge = tid < edges;
-  const int edge_at = tid < lay.head ? tid : n - lay.tail + (tid - lay.head);
-  const float edge = has_edge ? to_float(x[edge_at]) : -INFINITY;
-  if (tid == 0) count = 0;
-
-  uint32_t best = has_edge ? key_of(edge) : 0u;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (v0 + tid + i * DT < v1) {
-      float v[W];
-      unpack(raw[i], v, T());
-#pragma unroll
-      for (int e = 0; e < W; ++e) best = max(best, key_of(v[e]));
-    }
-  }
-  const int mine = min(k, (v1 - v0) * W + edges);  // entries this part can contribute
+  if (i < nv) m0 = Ord::largest(m0, st.row[i]);
+  const uint32_t best = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
 
   // Bound: at least `mine` elements have a key >= bound (0: all elements).
-  const int filled = __syncthreads_count(best != 0);
   uint32_t bound = 0;
-  if (filled >= mine && mine > 0) {
-    const uint32_t hi0 = block_reduce(best, red_u, Max());
-    const uint32_t lo0 = block_reduce(best ? best : 0xffffffffu, red_u, Min());
-    uint32_t lo = lo0, hi = hi0;  // count(>= lo) >= mine; the bound is <= hi
-    while (lo < hi) {
+  if (__syncthreads_count(best != 0) >= mine && mine > 0) {
+    uint32_t hi = block_reduce<DT>(best, red_u, Max());
+    uint32_t lo = block_reduce<DT>(best ? best : 0xffffffffu, red_u, Min());
+    while (lo < hi) {  // count(>= lo) >= mine; the bound is <= hi
       const uint32_t mid = lo + (hi - lo) / 2 + 1;
       const int got = __syncthreads_count(best >= mid);
       if (got >= mine) {
         lo = mid;
-        if (got <= mine + mine / 4 + 8) break;
+        if (got <= mine + mine / 8 + 4) break;
       } else {
         hi = mid - 1;
       }
@@ -227,96 +343,104 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   }
 
   int last_at = 0x7fffffff;  // elements equal to the bound count up to this position
+  auto taken = [&](uint32_t key, int at) { return key > bound || (key == bound && at <= last_at); };
   float m = 0.0f, s = 0.0f;  // the sum of what is not kept, as sum of 2^((x - m) c)
   for (int attempt = 0;; ++attempt) {
     // Everything not a candidate lies at or below the bound. A bound that cannot be an anchor
     // (infinite, NaN, a mask's value) leaves the sum to the code behind the ranking.
-    m = bound ? value_of(bound) : -INFINITY;
+    m = bound ? Ord::value(bound) : -INFINITY;
     const bool near = fabsf(m) < FAR;
     const float anchor = near ? -m * c : 0.0f;
-    s = 0.0f;
-    auto element = [&](float v, int at) {
-      const uint32_t key = key_of(v);
-      if (key > bound || (key == bound && at <= last_at)) {
-        const int pos = atomicAdd(&count, 1);
-        if (pos < TOP_CAP)
-          cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
-      } else if (near) {
-        s += exp2_approx(fmaf(v, c, anchor));
-      }
-    };
-    __syncthreads();
+    f32x2 acc = f2_pack(0.0f, 0.0f);
+    float odd = 0.0f;
+#pragma unroll 2
+    for (int j = tid; j < nv; j += DT) {
+      const uint4 q = st.row[j];
+      if (near && Ord::all_below(Ord::largest(Ord::kLow, q), m)) {
+        add_exponentials<T>(q, c, anchor, acc);
+      } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = v0 + tid + i * DT;
-      if (j < v1) {
-        float v[W];
-        unpack(raw[i], v, T());
-#pragma unroll
-        for (int e = 0; e < W; ++e) element(v[e], lay.head + j * W + e);
+        for (int e = 0; e < W; ++e) {
+          const uint32_t key = Ord::key(bits_at<T>(q, e));
+          const int at = st.position(j, e);
+          if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
+          if (taken(key, at)) {
+            const int pos = atomicAdd(&count, 1);
+            if (pos < TOP_CAP)
+              cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+          } else if (near) {
+            odd += exp2_approx(fmaf(Ord::value(key), c, anchor));
+          }
+        }
       }
     }
-    if (has_edge) element(edge, edge_at);
+    float s0, s1;
+    f2_unpack(acc, s0, s1);
+    s = s0 + s1 + odd;
     if (near) s *= exp2_approx(-fmaf(m, c, anchor));  // the anchor's own rounding
     __syncthreads();
     if (count <= TOP_CAP || attempt == 1) break;
-    // Too many candidates: the exact k-th largest key, then the position of the last element
-    // equal to it that still belongs to the k largest.
     auto count_if = [&](auto test) {
       int got = 0;
+      for (int j = tid; j < nv; j += DT) {
+        const uint4 q = st.row[j];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = v0 + tid + i * DT;
-        if (j < v1) {
-          float v[W];
-          unpack(raw[i], v, T());
-#pragma unroll
-          for (int e = 0; e < W; ++e) got += test(key_of(v[e]), lay.head + j * W + e) ? 1 : 0;
+        for (int e = 0; e < W; ++e) {
+          const int at = st.position(j, e);
+          if (static_cast<unsigned>(at) < static_cast<unsigned>(n))
+            got += test(Ord::key(bits_at<T>(q, e)), at) ? 1 : 0;
         }
       }
-      if (has_edge) got += test(key_of(edge), edge_at) ? 1 : 0;
-      return static_cast<int>(block_reduce(static_cast<uint32_t>(got), red_u, Sum()));
+      return static_cast<int>(block_reduce<DT>(static_cast<uint32_t>(got), red_u, Sum()));
     };
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = kth | (1u << bit);
-      if (count_if([&](uint32_t key, int) { return key >= trial; }) >= mine) kth = trial;
+    uint32_t lo = bound, hi = sizeof(T) == 4 ? 0xffffffffu : 0xffffu;
+    int got = TOP_CAP + 1;
+    while (lo < hi && got > TOP_CAP) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      const int above = count_if([&](uint32_t key, int) { return key >= mid; });
+      if (above >= mine) {
+        lo = mid;
+        got = above;
+      } else {
+        hi = mid - 1;
+      }
     }
-    const int need = mine - count_if([&](uint32_t key, int) { return key > kth; });
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if (count_if([&](uint32_t key, int at) { return key == kth && at <= mid; }) >= need) hi = mid;
-      else lo = mid + 1;
+    bound = lo;
+    if (got > TOP_CAP) {  // too many elements equal to the k-th largest: the first ones of them
+      const int need = mine - count_if([&](uint32_t key, int) { return key > lo; });
+      int a0 = 0, a1 = n - 1;
+      while (a0 < a1) {
+        const int mid = a0 + (a1 - a0) / 2;
+        if (count_if([&](uint32_t key, int at) { return key == lo && at <= mid; }) >= need) a1 = mid;
+        else a0 = mid + 1;
+      }
+      last_at = a0;
     }
-    bound = kth;
-    last_at = lo;
     __syncthreads();
     if (tid == 0) count = 0;
+    __syncthreads();
   }
-  const int found = count;
+  const int found = min(count, TOP_CAP);
 
-  // Rank of every candidate; the first `mine` in order go to top[].
-  uint32_t lost = 0;  // largest key of this thread's candidates that lose
-  uint32_t lost_mask = 0;
-#pragma unroll 1
-  for (int i = tid, q = 0; i < found; i += DT, ++q) {
-    const u64 me = cand[i];
+  // Rank of every candidate = number of larger ones (all are different: the position is part).
+  if (tid == 0 && (found & 1)) cand[found] = 0;  // found < TOP_CAP then; read in pairs below
+  __syncthreads();
+  for (int q = tid; q < found; q += DT) {
+    const u64 me = cand[q];
     int rank = 0;
-    for (int j = 0; j < found; ++j) rank += cand[j] > me ? 1 : 0;
-    if (rank < mine) {
-      top[rank] = me;
-    } else {
-      lost = max(lost, static_cast<uint32_t>(me >> 32));
-      lost_mask |= 1u << q;
+    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
+#pragma unroll 4
+    for (int j = 0; j < (found + 1) / 2; ++j) {
+      const ulonglong2 two = pairs[j];
+      rank += (two.x > me ? 1 : 0) + (two.y > me ? 1 : 0);
     }
+    sorted[rank] = me;
   }
-  s = block_reduce(s, red_f, Sum());
-  lost = block_reduce(lost, red_u, Max());  // its barriers also publish top[]
+  s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
   // Adds values (each thread's own, through `each`) whose largest key is `key` to the sum; none of
   // them lies below what is in the sum already.
   auto add_at = [&](uint32_t key, auto each) {
-    const float top_value = value_of(key);
+    const float top_value = Ord::value(key);
     if (!(top_value < INFINITY)) {  // +inf or NaN: so is the sum
       m = 0.0f;
       s = top_value;
@@ -325,47 +449,35 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     float t = 0.0f;
     if (top_value > -INFINITY) {
       each([&](float v) { t += exp2_approx((v - top_value) * c); });
-      t = block_reduce(t, red_f, Sum());
+      t = block_reduce<DT>(t, red_f, Sum());
       s = (s > 0.0f ? s * exp2_approx((m - top_value) * c) : s) + t;
       m = top_value;
     }
   };
-  if (lost) {
-    // The losing candidates are at or above the bound: their largest is the new anchor.
-    add_at(lost, [&](auto add) {
-#pragma unroll 1
-      for (int i = tid, q = 0; i < found; i += DT, ++q)
-        if (lost_mask >> q & 1) add(value_of(static_cast<uint32_t>(cand[i] >> 32)));
+  if (found > mine) {
+    // The losing candidates are at or above the bound: the first of them is the new anchor.
+    add_at(static_cast<uint32_t>(sorted[mine] >> 32), [&](auto add) {
+      for (int q = mine + tid; q < found; q += DT) add(Ord::value(static_cast<uint32_t>(sorted[q] >> 32)));
     });
   } else if (s < 1e-30f) {
     // Nothing, or all of it far below the bound: anchor at the largest of it.
-    auto below = [&](float v, int at) {
-      const uint32_t key = key_of(v);
-      return !(key > bound || (key == bound && at <= last_at)) ? key : 0u;
-    };
     auto walk = [&](auto visit) {
+      for (int j = tid; j < nv; j += DT) {
+        const uint4 q = st.row[j];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = v0 + tid + i * DT;
-        if (j < v1) {
-          float v[W];
-          unpack(raw[i], v, T());
-#pragma unroll
-          for (int e = 0; e < W; ++e) visit(v[e], lay.head + j * W + e);
+        for (int e = 0; e < W; ++e) {
+          const uint32_t key = Ord::key(bits_at<T>(q, e));
+          const int at = st.position(j, e);
+          if (static_cast<unsigned>(at) < static_cast<unsigned>(n) && !taken(key, at)) visit(key);
         }
       }
-      if (has_edge) visit(edge, edge_at);
     };
     uint32_t low = 0;
-    walk([&](float v, int at) { low = max(low, below(v, at)); });
-    low = block_reduce(low, red_u, Max());
+    walk([&](uint32_t key) { low = max(low, key); });
+    low = block_reduce<DT>(low, red_u, Max());
     s = 0.0f;
     if (low)
-      add_at(low, [&](auto add) {
-        walk([&](float v, int at) {
-          if (below(v, at)) add(v);
-        });
-      });
+      add_at(low, [&](auto add) { walk([&](uint32_t key) { add(Ord::value(key)); }); });
   }
 
   auto emit = [&](int rank, u64 entry) {
@@ -378,38 +490,35 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
                        : static_cast<float>(top_value * inv_t + log(static_cast<double>(sum)));
   };
   if (parts == 1) {
-    for (int i = tid; i < mine; i += DT) emit(i, top[i]);
-    if (tid == 0) rest[r] = log_of(m, s);
+    for (int q = tid; q < mine; q += DT) emit(q, sorted[q]);
+    if (tid == 0) rest[r] = gave_up ? NAN : log_of(m, s);
     return;
   }
 
   // The parts' sorted lists meet: an entry's place in the row is its place here plus the number
   // of larger entries in the other lists.
-  for (int i = tid; i < TOP_K_MAX; i += DT)
-    if (i >= mine) top[i] = 0;
+  __syncthreads();
+  for (int q = mine + tid; q < k; q += DT) sorted[q] = 0;
   cluster_sync_all();
-  u64* lists = cand;  // [parts][TOP_K_MAX], this CTA's candidates are no longer needed
-  static_assert(TOP_CAP >= MAX_PARTS * TOP_K_MAX, "the parts' lists take the candidates' place");
-  for (int i = tid; i < parts * k; i += DT) {
-    const int p = i / k, q = i % k;
+  u64* lists = reinterpret_cast<u64*>(row_smem);  // [parts][k]: the row is no longer needed
+  for (int q = tid; q < parts * k; q += DT) {
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];"
                  : "=l"(v)
-                 : "r"(mapa_shared(smem_u32(top + q), static_cast<uint32_t>(p))));
-    lists[p * TOP_K_MAX + q] = v;
+                 : "r"(mapa_shared(smem_u32(sorted + q % k), static_cast<uint32_t>(q / k))));
+    lists[q] = v;
   }
   __syncthreads();
   uint32_t out_key = 0;
-  u64 me = 0;
-  if (tid < mine) {
-    me = top[tid];
+  if (tid < mine) {  // k <= 256 <= DT
+    const u64 me = sorted[tid];
     int rank = tid;
     for (int p = 0; p < parts; ++p) {
       if (p == part) continue;
       int lo = 0, hi = k;  // first position whose entry is smaller
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (lists[p * TOP_K_MAX + mid] > me) lo = mid + 1;
+        if (lists[p * k + mid] > me) lo = mid + 1;
         else hi = mid;
       }
       rank += lo;
@@ -417,14 +526,15 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     if (rank < k) emit(rank, me);
     else out_key = static_cast<uint32_t>(me >> 32);
   }
-  const uint32_t high = block_reduce(out_key, red_u, Max());
+  const uint32_t high = block_reduce<DT>(out_key, red_u, Max());
   if (high)
     add_at(high, [&](auto add) {
-      if (out_key) add(value_of(out_key));
+      if (out_key) add(Ord::value(out_key));
     });
   if (tid == 0) {
     const uint32_t dst = mapa_shared(smem_u32(part_rest + part), 0);
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(m), "f"(s) : "memory");
+    const float sum = gave_up ? NAN : s;
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(m), "f"(sum) : "memory");
   }
   cluster_sync_all();  // also: no CTA leaves while another may read its list
   if (part == 0 && tid == 0) {
@@ -449,6 +559,8 @@ __device__ __forceinline__ int load_index(const void* p, int wide, long long i, 
   const long long v = wide ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
   return v >= 0 && v < n ? static_cast<int>(v) : -1;
 }
+
+constexpr int FT = 256;  // threads of the forward and backward kernels
 
 struct DistillParams {
   const void* values;
@@ -490,86 +602,99 @@ struct Running {
   }
 };
 
-// The student's exponentials are summed over the classes that are NOT kept (a bitmap in shared
-// memory marks the kept ones; one byte test per 8 bf16 elements), in one pass with a running
-// maximum. The at most k + 1 terms of the divergence are evaluated in 64 bits: where student and
-// teacher agree their first-order parts cancel, and so do q - p in the gradient. stats and slopes
-// leave nothing but one exponential per class to the backward pass.
+// The student's exponentials are summed over the classes that are NOT kept: the kept ones are taken
+// out of the row in shared memory (each entry writes its number over its class, one that finds
+// another's number there is listed twice; then -inf replaces the numbers). Every thread takes the
+// maximum of its own vectors and sums relative to it. The at most k + 1 terms of the divergence are
+// evaluated in 64 bits: where student and teacher agree their first-order parts cancel, and so do
+// q - p in the gradient. stats and slopes leave nothing but one exponential per class to the
+// backward pass.
 template <typename T>
-__global__ void __launch_bounds__(DT)
+__global__ void __launch_bounds__(FT)
 distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
+  constexpr int DT = FT, DW = DT / 32;
   constexpr int W = Vec<T>::W;
-  extern __shared__ uint32_t bitmap[];
+  using Ord = Order<T>;
+  using Tag = typename std::conditional<sizeof(T) == 4, uint32_t, unsigned short>::type;
+  extern __shared__ __align__(16) uint4 row_smem[];
   __shared__ double red_d[DW];
   __shared__ float4 red_run[DW];
   __shared__ float4 part_run[MAX_PARTS];
-  __shared__ int repeated;
+  __shared__ __align__(8) uint64_t bar_mem;
+  __shared__ int repeated, gave_up;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = p.parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long r = blockIdx.x / p.parts;
   const int n = p.n, k = p.k;
   const T* x = logits + r * p.ld;
-  const RowLayout<T> lay(x, n);
-  const int per = (lay.vectors + p.parts - 1) / p.parts;
-  const int v0 = min(part * per, lay.vectors), v1 = min(v0 + per, lay.vectors);
-  // Bit of element e: the part's vectors from bit W on, the edges in front of and behind them.
-  const int first = lay.head + v0 * W - W;
-  const int last = part == p.parts - 1 ? n : lay.head + v1 * W;
-  const int words = (last - first + 31) / 32;
-  for (int i = tid; i < words; i += DT) bitmap[i] = 0;
-  if (tid == 0) repeated = 0;
+  const uint32_t bar = smem_u32(&bar_mem);
+  const StagedRow<T, DT> st(x, n, part, p.parts, row_smem, bar);
+  if (tid == 0) repeated = gave_up = 0;
+  // The first DT entries stay in registers: class, teacher's logit, student's logit.
+  const double inv_t = 1.0 / p.temperature;
+  int my_at = -1;
+  double my_t = -INFINITY, my_z = -INFINITY;
+  if (tid < k) {
+    my_at = load_index(p.indices, p.indices_wide, r * p.ld_indices + tid, n);
+    my_t = load_value(p.values, p.values_dtype, r * p.ld_values + tid) * inv_t;
+    if (my_at >= 0) my_z = to_float(x[my_at]) * inv_t;
+  }
+  const float c = p.c;
+  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
+  __syncthreads();
+  if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
+  auto class_at = [&](int i) {
+    return i == tid ? my_at : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+  };
+  Tag* tags = reinterpret_cast<Tag*>(row_smem);
+  const int base = st.v0 * W - st.off, span = (st.v1 - st.v0) * W;
+  for (int i = tid; i < k; i += DT) {
+    const int at = class_at(i) - base;
+    if (class_at(i) >= 0 && at >= 0 && at < span) tags[at] = static_cast<Tag>(i);
+  }
   __syncthreads();
   for (int i = tid; i < k; i += DT) {
-    const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
-    const bool here = at >= (part == 0 ? 0 : first + W) && at < last;
-    if (here) {
-      const int b = at - first;
-      if (atomicOr(&bitmap[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) repeated = 1;
-    }
+    const int at = class_at(i) - base;
+    if (class_at(i) >= 0 && at >= 0 && at < span && tags[at] != static_cast<Tag>(i)) repeated = 1;
+  }
+  __syncthreads();
+  for (int i = tid; i < k; i += DT) {
+    const int at = class_at(i) - base;
+    if (class_at(i) >= 0 && at >= 0 && at < span) reinterpret_cast<T*>(row_smem)[at] = from_float<T>(-INFINITY);
   }
   __syncthreads();
 
   Running run = {-INFINITY, INFINITY, 0.0f};
-  const float c = p.c;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + lay.head);
-  const uint8_t* marks = reinterpret_cast<const uint8_t*>(bitmap);
-  constexpr int U = 4;
-  for (int j0 = v0 + tid; j0 < v1; j0 += U * DT) {
-    uint4 raw[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (j0 + i * DT < v1) raw[i] = __ldg(xv + j0 + i * DT);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int j = j0 + i * DT;
-      if (j >= v1) break;
-      float v[W];
-      unpack(raw[i], v, T());
-      const int b = (j - v0 + 1) * W;
-      const uint32_t mark = (marks[b >> 3] >> (b & 7)) & ((1u << W) - 1u);
-      if (mark) {
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          if (mark >> e & 1) v[e] = -INFINITY;
-      }
-      float top = v[0];
-#pragma unroll
-      for (int e = 1; e < W; ++e) top = fmaxf(top, v[e]);
-      run.raise(top, c);
-      if (!(top == -INFINITY)) {
-#pragma unroll
-        for (int e = 0; e < W; ++e) run.s += run.of(v[e], c);
-      }
-    }
-  }
+  const int nv = st.v1 - st.v0;
   {
-    const int edges = (part == 0 ? lay.head : 0) + (part == p.parts - 1 ? lay.tail : 0);
-    if (tid < edges) {
-      const int at = part == 0 && tid < lay.head ? tid : n - lay.tail + (tid - (part == 0 ? lay.head : 0));
-      const int b = at - first;
-      const float v = bitmap[b >> 5] >> (b & 31) & 1 ? -INFINITY : to_float(x[at]);
-      run.raise(v, c);
-      if (!(v == -INFINITY)) run.s += run.of(v, c);
+    uint32_t m0 = Ord::kLow, m1 = Ord::kLow;
+    int i = tid;
+    for (; i + DT < nv; i += 2 * DT) {
+      m0 = Ord::largest(m0, st.row[i]);
+      m1 = Ord::largest(m1, st.row[i + DT]);
+    }
+    if (i < nv) m0 = Ord::largest(m0, st.row[i]);
+    const uint32_t best = max(Ord::key_of_largest(m0), Ord::key_of_largest(m1));
+    const float top = Ord::value(best);
+    run.m = top;  // NaN: the sum below is NaN
+    run.a = -top * c;
+    if (run.far()) {
+      if (top != -INFINITY) {
+        for (int j = tid; j < nv; j += DT) {
+          float v[W];
+          unpack(st.row[j], v, T());
+#pragma unroll
+          for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - top) * c);
+        }
+      }
+      if (top != top) run.m = 0.0f, run.a = 0.0f;
+    } else {
+      f32x2 acc = f2_pack(0.0f, 0.0f);
+#pragma unroll 2
+      for (int j = tid; j < nv; j += DT) add_exponentials<T>(st.row[j], c, run.a, acc);
+      float s0, s1;
+      f2_unpack(acc, s0, s1);
+      run.s = s0 + s1;
     }
   }
 #pragma unroll
@@ -587,8 +712,9 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   if (p.parts > 1) {
     if (tid == 0) {
       const uint32_t dst = mapa_shared(smem_u32(part_run + part), 0);
+      const int flags = repeated | (gave_up << 1);
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(run.m),
-                   "f"(run.a), "f"(run.s), "f"(__int_as_float(repeated))
+                   "f"(run.a), "f"(run.s), "f"(__int_as_float(flags))
                    : "memory");
     }
     cluster_sync_all();
@@ -599,26 +725,29 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
       run.join(part_run[i].x, part_run[i].y, part_run[i].z, c);
       any |= __float_as_int(part_run[i].w);
     }
-    if (tid == 0) repeated = any;
+    if (tid == 0) repeated = any & 1, gave_up = any >> 1;
     __syncthreads();
   }
 
   // Natural-log units from here on, in 64 bits, maxima and sums kept apart (a maximum of the size
   // of a mask's value would swallow the logarithm of its sum). zm, zs: the classes not kept;
   // fmaf(m, c, a) is what rounding the anchor to fp32 left over.
-  const double inv_t = 1.0 / p.temperature;
   const bool some = run.s != 0.0f;
   const double zm = some ? run.m * inv_t : -INFINITY;
   const double zs = run.far() ? run.s : run.s * exp2(-static_cast<double>(fmaf(run.m, c, run.a)));
-  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
   auto entry = [&](int i, double& t, double& z) {  // teacher's and student's logit; false: left out
-    const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+    const int at = class_at(i);
     if (at < 0) return false;
     if (repeated)  // the first entry of a class counts
       for (int j = 0; j < i; ++j)
         if (load_index(p.indices, p.indices_wide, r * p.ld_indices + j, n) == at) return false;
-    t = load_value(p.values, p.values_dtype, r * p.ld_values + i) * inv_t;
-    z = to_float(x[at]) * inv_t;
+    if (i == tid) {
+      t = my_t;
+      z = my_z;
+    } else {
+      t = load_value(p.values, p.values_dtype, r * p.ld_values + i) * inv_t;
+      z = to_float(x[at]) * inv_t;
+    }
     return true;
   };
   double t_max = tr, z_max = zm;
@@ -628,8 +757,8 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     t_max = Max()(t, t_max);
     z_max = Max()(z, z_max);
   }
-  t_max = block_reduce(t_max, red_d, Max());
-  z_max = block_reduce(z_max, red_d, Max());
+  t_max = block_reduce<DT>(t_max, red_d, Max());
+  z_max = block_reduce<DT>(z_max, red_d, Max());
   auto part_of = [](double v, double top) { return v == -INFINITY ? 0.0 : exp(v - top); };
   double t_sum = 0.0, z_sum = 0.0;
   for (int i = tid; i < k; i += DT) {
@@ -638,8 +767,8 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     t_sum += part_of(t, t_max);
     z_sum += part_of(z, z_max);
   }
-  t_sum = block_reduce(t_sum, red_d, Sum()) + part_of(tr, t_max);
-  z_sum = block_reduce(z_sum, red_d, Sum()) + part_of(zm, z_max) * zs;
+  t_sum = block_reduce<DT>(t_sum, red_d, Sum()) + part_of(tr, t_max);
+  z_sum = block_reduce<DT>(z_sum, red_d, Sum()) + part_of(zm, z_max) * zs;
   const double t_log = log(t_sum), z_log = log(z_sum);
   // Teacher's and student's probability of an outcome, and its term of the divergence. A teacher
   // without any mass (no entry left, no rest) teaches nothing.
@@ -663,9 +792,9 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   }
   double q_rest = 0.0, p_rest = 0.0;
   if (tid == 0) p_rest = outcome(tr, zm, zs, q_rest);
-  loss = block_reduce(loss, red_d, Sum());
+  loss = block_reduce<DT>(loss, red_d, Sum());
   if (tid == 0) {
-    p.loss[r] = static_cast<float>(loss * p.temperature * p.temperature);
+    p.loss[r] = gave_up ? NAN : static_cast<float>(loss * p.temperature * p.temperature);
     // Gradient of a class that is not kept: q_j (1 - p_rest / q_rest).
     p.stats[r] = make_float2(run.m, some ? static_cast<float>((q_rest - p_rest) / run.s) : 0.0f);
   }
@@ -675,12 +804,13 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
 // saved slope for the others. One read and one write of the row; a row whose d_loss is zero (padding)
 // is zeroed without being read. Columns n .. n_pad (row padding of the gradient) get zeros.
 template <typename T>
-__global__ void __launch_bounds__(DT)
+__global__ void __launch_bounds__(FT)
 distill_bwd_kernel(const T* __restrict__ logits, const void* __restrict__ indices, int indices_wide,
                    long long ld_indices, const float2* __restrict__ stats,
                    const float* __restrict__ slopes, const float* __restrict__ d_loss,
                    long long d_loss_stride, T* __restrict__ grad, long long ld, long long ld_grad,
                    int n, int n_pad, int k, int parts, float c, float temperature) {
+  constexpr int DT = FT;
   constexpr int W = Vec<T>::W;
   const int tid = threadIdx.x;
   const long long r = blockIdx.x / parts;
@@ -751,9 +881,21 @@ int check_launch() {
   return 0;
 }
 
+constexpr int MAX_PART_BYTES = 176 * 1024;  // of a row in one CTA's shared memory
+
 template <typename... Params, typename... Args>
-int launch_clusters(void (*kernel)(Params...), int64_t rows, int parts, size_t smem, cudaStream_t stream,
-                    Args... args) {
+int launch_clusters(void (*kernel)(Params...), int64_t rows, int parts, int threads, size_t smem,
+                    cudaStream_t stream, Args... args) {
+  if (smem > 24 * 1024) {  // may pass the default limit together with the static part
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               MAX_PART_BYTES + 64);
+    if (e != cudaSuccess) {
+      set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+      cudaGetLastError();
+      return -4;
+    }
+  }
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cudaLaunchAttribute attr;
@@ -763,7 +905,7 @@ int launch_clusters(void (*kernel)(Params...), int64_t rows, int parts, size_t s
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
-  cfg.blockDim = dim3(DT);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
@@ -791,31 +933,32 @@ int choose_parts(int64_t rows, int vectors, int least) {
   return parts;
 }
 
-constexpr int TOP_NV_MAX = 12;
 constexpr int64_t MAX_ROWS = 1 << 27;
+
+// CTAs per row of the staged kernels and the shared memory of each (bytes of its vectors; a row may
+// start anywhere within 16 bytes, which adds a vector).
+int staged_parts(int64_t rows, int64_t n, int itemsize, int least, size_t* bytes) {
+  const int64_t vectors = (n * itemsize + 15) / 16 + 1;
+  int parts = choose_parts(rows, static_cast<int>(vectors), least);
+  while (parts < MAX_PARTS && (vectors + parts - 1) / parts * 16 > MAX_PART_BYTES) parts *= 2;
+  *bytes = static_cast<size_t>((vectors + parts - 1) / parts * 16);
+  return parts;
+}
 
 template <typename T>
 int top_logits(const void* logits, int64_t rows, int64_t n, int64_t ld, int64_t k, double temperature,
                void* values, int32_t* indices, float* rest, cudaStream_t stream) {
-  constexpr int W = Vec<T>::W;
-  const int vectors = static_cast<int>(n / W);
-  int parts = choose_parts(rows, vectors, DT);
-  while (parts < MAX_PARTS && (vectors + parts - 1) / parts > TOP_NV_MAX * DT) parts *= 2;
-  const int nv = ((vectors + parts - 1) / parts + DT - 1) / DT;
+  size_t smem = 0;
+  const int parts = staged_parts(rows, n, sizeof(T), 256, &smem);
+  if (parts > 1 && smem < static_cast<size_t>(parts * k * 8)) smem = static_cast<size_t>(parts * k * 8);
   const float c = static_cast<float>(1.4426950408889634 / temperature);
   const double inv_t = 1.0 / temperature;
-#define VMOE_TOP(NV)                                                                              \
-  return launch_clusters(top_logits_kernel<T, NV>, rows, parts, 0, stream,                        \
-                         static_cast<const T*>(logits), static_cast<long long>(ld),               \
-                         static_cast<int>(n), static_cast<int>(k), c, inv_t, parts,               \
-                         static_cast<T*>(values), indices, rest)
-  if (nv <= 1) VMOE_TOP(1);
-  if (nv <= 2) VMOE_TOP(2);
-  if (nv <= 4) VMOE_TOP(4);
-  if (nv <= 8) VMOE_TOP(8);
-  if (nv <= TOP_NV_MAX) VMOE_TOP(TOP_NV_MAX);
-#undef VMOE_TOP
-  return bad("top_logits: too many classes");
+  // More threads give more maxima to bound the k-th largest value with.
+  const int threads = k > 96 ? 512 : 256;
+  auto kernel = threads == 512 ? top_logits_kernel<T, 512> : top_logits_kernel<T, 256>;
+  return launch_clusters(kernel, rows, parts, threads, smem, stream, static_cast<const T*>(logits),
+                         static_cast<long long>(ld), static_cast<int>(n), static_cast<int>(k), c, inv_t,
+                         parts, static_cast<T*>(values), indices, rest);
 }
 
 }  // namespace
@@ -824,7 +967,7 @@ int top_logits(const void* logits, int64_t rows, int64_t n, int64_t ld, int64_t 
 using namespace vmoe;
 
 extern "C" int64_t vmoe_top_logits_max_classes(int32_t dtype) {
-  return static_cast<int64_t>(MAX_PARTS) * TOP_NV_MAX * DT * (dtype == 0 ? 4 : 8);
+  return static_cast<int64_t>(MAX_PARTS) * MAX_PART_BYTES / (dtype == 0 ? 4 : 2) - 64;
 }
 
 extern "C" int vmoe_top_logits(const void* logits, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
@@ -844,13 +987,13 @@ extern "C" int vmoe_top_logits(const void* logits, int32_t dtype, int64_t rows, 
   return bad("top_logits: unknown dtype");
 }
 
-extern "C" int64_t vmoe_distill_max_classes(void) { return 1 << 18; }
+extern "C" int64_t vmoe_distill_max_classes(int32_t dtype) { return vmoe_top_logits_max_classes(dtype); }
 
 extern "C" int vmoe_distill_fwd(const VmoeDistillArgs* a, vmoe_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (a->rows == 0) return 0;
-  if (a->rows < 0 || a->rows > MAX_ROWS || a->n < 1 || a->n > vmoe_distill_max_classes() || a->k < 1 ||
-      a->k > (1 << 20))
+  if (a->rows < 0 || a->rows > MAX_ROWS || a->n < 1 || a->n > vmoe_distill_max_classes(a->dtype) ||
+      a->k < 1 || a->k > 65535)
     return bad("distill: rows, classes or kept classes out of range");
   if (!(a->temperature > 0.0)) return bad("distill: temperature must be positive");
   DistillParams p;
@@ -869,15 +1012,14 @@ extern "C" int vmoe_distill_fwd(const VmoeDistillArgs* a, vmoe_stream_t stream_)
   p.indices_wide = a->indices_wide;
   p.c = static_cast<float>(1.4426950408889634 / a->temperature);
   p.temperature = a->temperature;
-  const int width = a->dtype == 0 ? 4 : 8;
-  p.parts = choose_parts(a->rows, static_cast<int>(a->n / width), 2 * DT);
-  const size_t smem = ((a->n / width + p.parts - 1) / p.parts + 4) * width / 8 + 8;
+  size_t smem = 0;
+  p.parts = staged_parts(a->rows, a->n, a->dtype == 0 ? 4 : 2, 2 * FT, &smem);
   switch (a->dtype) {
-    case 0: return launch_clusters(distill_fwd_kernel<float>, a->rows, p.parts, smem, stream,
+    case 0: return launch_clusters(distill_fwd_kernel<float>, a->rows, p.parts, FT, smem, stream,
                                    static_cast<const float*>(a->logits), p);
-    case 1: return launch_clusters(distill_fwd_kernel<__nv_bfloat16>, a->rows, p.parts, smem, stream,
+    case 1: return launch_clusters(distill_fwd_kernel<__nv_bfloat16>, a->rows, p.parts, FT, smem, stream,
                                    static_cast<const __nv_bfloat16*>(a->logits), p);
-    case 2: return launch_clusters(distill_fwd_kernel<__half>, a->rows, p.parts, smem, stream,
+    case 2: return launch_clusters(distill_fwd_kernel<__half>, a->rows, p.parts, FT, smem, stream,
                                    static_cast<const __half*>(a->logits), p);
   }
   return bad("distill: unknown dtype");
@@ -887,7 +1029,7 @@ extern "C" int vmoe_distill_bwd(const VmoeDistillArgs* a, const float* d_loss, i
                                 void* grad, int64_t ld_grad, int64_t n_pad, vmoe_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (a->rows == 0) return 0;
-  if (a->rows < 0 || a->rows > MAX_ROWS || a->n < 1 || a->n > vmoe_distill_max_classes() ||
+  if (a->rows < 0 || a->rows > MAX_ROWS || a->n < 1 || a->n > vmoe_distill_max_classes(a->dtype) ||
       n_pad < a->n || n_pad > ld_grad)
     return bad("distill: rows or classes out of range");
   const int itemsize = a->dtype == 0 ? 4 : 2;
@@ -896,11 +1038,11 @@ extern "C" int vmoe_distill_bwd(const VmoeDistillArgs* a, const float* d_loss, i
   if ((reinterpret_cast<uintptr_t>(a->logits) - reinterpret_cast<uintptr_t>(grad)) % 16 ||
       ((a->ld - ld_grad) * itemsize) % 16)
     return bad("distill: gradient rows must have the alignment of the logits' rows");
-  const int parts = choose_parts(a->rows, static_cast<int>(a->n / (16 / itemsize)), DT);
+  const int parts = choose_parts(a->rows, static_cast<int>(a->n / (16 / itemsize)), FT);
   const unsigned grid = static_cast<unsigned>(a->rows * parts);
   const float c = static_cast<float>(1.4426950408889634 / a->temperature);
 #define VMOE_DISTILL_BWD(T)                                                                         \
-  distill_bwd_kernel<T><<<grid, DT, 0, stream>>>(                                                   \
+  distill_bwd_kernel<T><<<grid, FT, 0, stream>>>(                                                   \
       static_cast<const T*>(a->logits), a->indices, a->indices_wide, a->ld_indices,                 \
       reinterpret_cast<const float2*>(a->stats), a->slopes, d_loss, d_loss_stride,                  \
       static_cast<T*>(grad), a->ld, ld_grad, static_cast<int>(a->n), static_cast<int>(n_pad),       \

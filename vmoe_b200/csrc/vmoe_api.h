@@ -216,7 +216,7 @@ VMOE_API int vmoe_xent(int32_t kind, const void* logits, const void* labels, int
 
 // ----------------------------------------------------------------------------- distillation
 // dtype codes of logits and values: 0 fp32, 1 bf16, 2 fp16.
-// The k <= 256 largest logits of every row, sorted (ties: lower class first; NaN above +inf):
+// Rows of up to vmoe_*_max_classes(dtype) classes. The k <= 256 largest logits of every row, sorted (ties: lower class first; NaN above +inf):
 // values (rows, k) in the logits' type, indices (rows, k), and rest (rows) = log-sum-exp of
 // logits / temperature over all the other classes (-inf when there are none).
 VMOE_API int64_t vmoe_top_logits_max_classes(int32_t dtype);
@@ -244,7 +244,7 @@ typedef struct VmoeDistillArgs {
   int32_t dtype, values_dtype;
   int32_t indices_wide;               // 0: int32, 1: int64
 } VmoeDistillArgs;
-VMOE_API int64_t vmoe_distill_max_classes(void);
+VMOE_API int64_t vmoe_distill_max_classes(int32_t dtype);
 VMOE_API int vmoe_distill_fwd(const VmoeDistillArgs* args, vmoe_stream_t stream);
 VMOE_API int vmoe_distill_bwd(const VmoeDistillArgs* args, const float* d_loss,
                               int64_t d_loss_stride, void* grad, int64_t ld_grad, int64_t n_pad,

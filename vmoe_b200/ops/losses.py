@@ -263,7 +263,8 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
     if t is not None and t.device != logits.device:
       raise ValueError(f"distill_xent: {name} is on {t.device}, logits on {logits.device}")
   values, rest = values.detach(), None if rest is None else rest.detach()
-  if _on_kernels(logits) and n <= _lib.lib().vmoe_distill_max_classes():
+  if (_on_kernels(logits) and values.shape[1] <= 65535 and
+      n <= _lib.lib().vmoe_distill_max_classes(ctypes.c_int32(_FLOAT_CODES[logits.dtype]))):
     if values.dtype not in _FLOAT_CODES:
       values = values.float()
     if rest is not None:
