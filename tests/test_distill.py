@@ -376,3 +376,19 @@ def test_distill_side_stream_and_graph_replay():
     buf.copy_(src)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@gpu
+@pytest.mark.parametrize("n,k", [(21843, 64), (50021, 200), (900, 256)])
+def test_results_do_not_depend_on_the_run(n, k):
+  x = make(64, n, torch.bfloat16, device="cuda")
+  y = make(64, n, torch.bfloat16, seed=8, device="cuda").requires_grad_()
+
+  def step():
+    top = losses.top_logits(x, k)
+    loss = losses.distill_xent(y, *top)
+    return (*top, loss.detach(), *torch.autograd.grad(loss.sum(), y))
+
+  first = step()
+  for _ in range(5):
+    assert all(torch.equal(a, b) for a, b in zip(first, step()))

@@ -172,19 +172,22 @@ __device__ __forceinline__ uint32_t bits_at(const uint4& q, int e) {
   return e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
 }
 
-// Sum of 2^(x c + a) over a vector.
+// Sum of 2^(x c + a) over a vector, as two partial sums.
 template <typename T>
-__device__ __forceinline__ void add_exponentials(const uint4& q, float c, float a, f32x2& sum) {
+__device__ __forceinline__ f32x2 exponentials(const uint4& q, float c, float a) {
   constexpr int W = Vec<T>::W;
   float v[W];
   unpack(q, v, T());
   const f32x2 cc = f2_pack(c, c), aa = f2_pack(a, a);
+  f32x2 sum = 0;  // two zeros
 #pragma unroll
   for (int e = 0; e < W; e += 2) {
     float t0, t1;
     f2_unpack(f2_fma(f2_pack(v[e], v[e + 1]), cc, aa), t0, t1);
-    sum = f2_add(sum, f2_pack(exp2_approx(t0), exp2_approx(t1)));
+    const f32x2 two = f2_pack(exp2_approx(t0), exp2_approx(t1));
+    sum = e == 0 ? two : f2_add(sum, two);
   }
+  return sum;
 }
 
 // Values beyond this are not multiplied by log2(e) / temperature before the row's anchor is taken
@@ -225,9 +228,6 @@ struct Sum {
 struct Max {
   __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
   __device__ __forceinline__ double operator()(double a, double b) const { return a > b || a != a ? a : b; }
-};
-struct Min {
-  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
 };
 
 // The vectors v0 .. v1 - 1 of a row that belong to this CTA, on their way to shared memory. Vector j
@@ -274,24 +274,32 @@ struct StagedRow {
     return v1 > v0 ? min(n, v1 * W - off) - max(0, v0 * W - off) : 0;
   }
   __device__ __forceinline__ int position(int i, int e) const { return (v0 + i) * W + e - off; }
+  __device__ __forceinline__ bool holds(int position) const {
+    return position >= 0 && position < n && position + off >= v0 * W && position + off < v1 * W;
+  }
+  __device__ __forceinline__ T at(int position) const {
+    return reinterpret_cast<const T*>(row)[position + off - v0 * W];
+  }
 };
 
 // ------------------------------------------------------------------------------- top logits
 constexpr int TOP_CAP = 1024;  // candidates that shared memory holds
 constexpr int TOP_K_MAX = 256;
 
-// The k largest of the threads' maxima (found by bisection on their order keys, one block-wide count
-// per step) bound the k-th largest value from below, so everything not below that bound is a
-// candidate: somewhat more than k of them for values in no particular order. Where there are too
-// many (more kept than threads, rows of equal values) the bisection goes on over all values, and
-// over positions among equal ones. Candidates are ranked by counting the larger ones. The pass that
-// collects them also sums the exponentials of everything else relative to the bound; candidates
-// that lose and a sum that underflows get anchors of their own, so that `rest` is right however far
-// below the kept values it lies. All sums have a fixed order.
+// The k largest of the threads' maxima (found by one warp's bisection on their order keys) bound the
+// k-th largest value from below, so everything not below that bound is a candidate: somewhat more
+// than k of them for values in no particular order. Where there are too many (more kept than
+// threads, rows of equal values) the bisection goes on over all values, and over positions among
+// equal ones. The second pass over the row sums the exponentials relative to the bound and only
+// lists the vectors that hold a candidate: with some 100 candidates in 2700 vectors nearly every
+// warp would run through the code for them at every step. They are taken apart afterwards, one per
+// thread, and ranked by counting the larger ones. Candidates that lose and a sum that underflows get
+// anchors of their own, so that `rest` is right however far below the kept values it lies. Sums do not
+// depend on the order in which threads run.
 template <typename T, int DT>
 __global__ void __launch_bounds__(DT)
 top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, float c, double inv_t,
-                  int parts, T* __restrict__ values, int* __restrict__ indices,
+                  int parts, int list_offset, T* __restrict__ values, int* __restrict__ indices,
                   float* __restrict__ rest) {
   constexpr int W = Vec<T>::W;
   using Ord = Order<T>;
@@ -302,7 +310,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   __shared__ float red_f[DT / 32];
   __shared__ float2 part_rest[MAX_PARTS];
   __shared__ __align__(8) uint64_t bar_mem;
-  __shared__ int count, gave_up;
+  __shared__ int count, hot_count, gave_up;
+  __shared__ uint32_t first_bound;
+  __shared__ u64 odd_sum;
   const int tid = threadIdx.x;
   const int part = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long r = blockIdx.x / parts;
@@ -311,7 +321,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   const StagedRow<T, DT> st(x, n, part, parts, row_smem, bar);
   const int nv = st.v1 - st.v0;
   const int mine = min(k, st.elements());  // entries this part can contribute
-  if (tid == 0) count = gave_up = 0;
+  if (tid == 0) count = hot_count = gave_up = 0, odd_sum = 0;
   __syncthreads();
   if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
 
@@ -322,16 +332,30 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     m1 = Ord::largest(m1, st.row[i + DT]);
   }
   if (i < nv) m0 = Ord::largest(m0, st.row[i]);
-  const uint32_t best = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(cand);
+  keys[tid] = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
+  __syncthreads();
 
   // Bound: at least `mine` elements have a key >= bound (0: all elements).
-  uint32_t bound = 0;
-  if (__syncthreads_count(best != 0) >= mine && mine > 0) {
-    uint32_t hi = block_reduce<DT>(best, red_u, Max());
-    uint32_t lo = block_reduce<DT>(best ? best : 0xffffffffu, red_u, Min());
+  if (tid < 32) {
+    uint32_t own[DT / 32], lo = 0xffffffffu, hi = 0;
+    int filled = 0;
+#pragma unroll
+    for (int q = 0; q < DT / 32; ++q) {
+      own[q] = keys[tid + 32 * q];
+      hi = max(hi, own[q]);
+      if (own[q]) lo = min(lo, own[q]), ++filled;
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    filled = __reduce_add_sync(0xffffffffu, filled);
+    if (filled < mine || mine == 0) lo = hi = 0;
     while (lo < hi) {  // count(>= lo) >= mine; the bound is <= hi
       const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      const int got = __syncthreads_count(best >= mid);
+      int got = 0;
+#pragma unroll
+      for (int q = 0; q < DT / 32; ++q) got += own[q] >= mid ? 1 : 0;
+      got = __reduce_add_sync(0xffffffffu, got);
       if (got >= mine) {
         lo = mid;
         if (got <= mine + mine / 8 + 4) break;
@@ -339,47 +363,60 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
         hi = mid - 1;
       }
     }
-    bound = lo;
+    if (tid == 0) first_bound = lo;
   }
+  __syncthreads();
+  uint32_t bound = first_bound;
 
   int last_at = 0x7fffffff;  // elements equal to the bound count up to this position
   auto taken = [&](uint32_t key, int at) { return key > bound || (key == bound && at <= last_at); };
   float m = 0.0f, s = 0.0f;  // the sum of what is not kept, as sum of 2^((x - m) c)
+  int* hot = reinterpret_cast<int*>(sorted);  // vectors that hold candidates
   for (int attempt = 0;; ++attempt) {
     // Everything not a candidate lies at or below the bound. A bound that cannot be an anchor
     // (infinite, NaN, a mask's value) leaves the sum to the code behind the ranking.
     m = bound ? Ord::value(bound) : -INFINITY;
     const bool near = fabsf(m) < FAR;
     const float anchor = near ? -m * c : 0.0f;
-    f32x2 acc = f2_pack(0.0f, 0.0f);
-    float odd = 0.0f;
+    f32x2 acc = 0;
+    u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-50
+    auto take_apart = [&](int j, const uint4& q) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const uint32_t key = Ord::key(bits_at<T>(q, e));
+        const int at = st.position(j, e);
+        if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
+        if (taken(key, at)) {
+          const int pos = atomicAdd(&count, 1);
+          if (pos < TOP_CAP)
+            cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+        } else if (near) {
+          odd += __float2ull_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p50f);
+        }
+      }
+    };
 #pragma unroll 2
     for (int j = tid; j < nv; j += DT) {
       const uint4 q = st.row[j];
-      if (near && Ord::all_below(Ord::largest(Ord::kLow, q), m)) {
-        add_exponentials<T>(q, c, anchor, acc);
-      } else {
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const uint32_t key = Ord::key(bits_at<T>(q, e));
-          const int at = st.position(j, e);
-          if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
-          if (taken(key, at)) {
-            const int pos = atomicAdd(&count, 1);
-            if (pos < TOP_CAP)
-              cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
-          } else if (near) {
-            odd += exp2_approx(fmaf(Ord::value(key), c, anchor));
-          }
-        }
+      const f32x2 sum = exponentials<T>(q, c, anchor);
+      if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) {
+        acc = f2_add(acc, sum);
+      } else if (attempt == 0) {
+        const int pos = atomicAdd(&hot_count, 1);
+        if (pos < TOP_CAP) hot[pos] = j;
+      } else {  // exact bounds: any number of vectors may hold values equal to the bound
+        take_apart(j, q);
       }
     }
+    __syncthreads();
+    if (hot_count <= TOP_CAP)
+      for (int h = tid; h < hot_count; h += DT) take_apart(hot[h], st.row[hot[h]]);
+    if (odd) atomicAdd(&odd_sum, odd);  // integers: the order does not matter
     float s0, s1;
     f2_unpack(acc, s0, s1);
-    s = s0 + s1 + odd;
-    if (near) s *= exp2_approx(-fmaf(m, c, anchor));  // the anchor's own rounding
+    s = near ? s0 + s1 : 0.0f;
     __syncthreads();
-    if (count <= TOP_CAP || attempt == 1) break;
+    if ((hot_count <= TOP_CAP && count <= TOP_CAP) || attempt == 1) break;
     auto count_if = [&](auto test) {
       int got = 0;
       for (int j = tid; j < nv; j += DT) {
@@ -417,10 +454,10 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
       last_at = a0;
     }
     __syncthreads();
-    if (tid == 0) count = 0;
+    if (tid == 0) count = hot_count = 0, odd_sum = 0;
     __syncthreads();
   }
-  const int found = min(count, TOP_CAP);
+  const int found = min(count, TOP_CAP);  // >= mine
 
   // Rank of every candidate = number of larger ones (all are different: the position is part).
   if (tid == 0 && (found & 1)) cand[found] = 0;  // found < TOP_CAP then; read in pairs below
@@ -437,6 +474,8 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     sorted[rank] = me;
   }
   s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
+  if (fabsf(m) < FAR)  // the last factor takes the rounding of m c back
+    s = (s + static_cast<float>(odd_sum) * 0x1p-50f) * exp2_approx(-fmaf(m, c, -m * c));
   // Adds values (each thread's own, through `each`) whose largest key is `key` to the sum; none of
   // them lies below what is in the sum already.
   auto add_at = [&](uint32_t key, auto each) {
@@ -455,12 +494,24 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     }
   };
   if (found > mine) {
-    // The losing candidates are at or above the bound: the first of them is the new anchor.
-    add_at(static_cast<uint32_t>(sorted[mine] >> 32), [&](auto add) {
-      for (int q = mine + tid; q < found; q += DT) add(Ord::value(static_cast<uint32_t>(sorted[q] >> 32)));
-    });
-  } else if (s < 1e-30f) {
-    // Nothing, or all of it far below the bound: anchor at the largest of it.
+    // The losing candidates are at or above the bound: the first of them is the new anchor. They are
+    // few: the first warp adds them up (only thread 0 needs the sum).
+    const float top_value = Ord::value(static_cast<uint32_t>(sorted[mine] >> 32));
+    if (!(top_value < INFINITY)) {
+      m = 0.0f;
+      s = top_value;
+    } else if (tid < 32 && top_value > -INFINITY) {
+      float t = 0.0f;
+      for (int q = mine + tid; q < found; q += 32)
+        t += exp2_approx((Ord::value(static_cast<uint32_t>(sorted[q] >> 32)) - top_value) * c);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      s = (s > 0.0f ? s * exp2_approx((m - top_value) * c) : s) + t;
+      m = top_value;
+    }
+  } else if (s < 1e-8f) {
+    // Nothing, or all of it far below the bound (where the units of odd_sum and, further down, fp32
+    // itself would show): anchor at the largest of it.
     auto walk = [&](auto visit) {
       for (int j = tid; j < nv; j += DT) {
         const uint4 q = st.row[j];
@@ -482,8 +533,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
 
   auto emit = [&](int rank, u64 entry) {
     const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(entry));
+    if (!st.holds(at)) return;  // cannot be; keeps a wrong entry from reading elsewhere
     indices[r * k + rank] = at;
-    values[r * k + rank] = x[at];
+    values[r * k + rank] = st.at(at);
   };
   auto log_of = [&](float top_value, float sum) {
     return sum == 0.0f ? -INFINITY
@@ -500,7 +552,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   __syncthreads();
   for (int q = mine + tid; q < k; q += DT) sorted[q] = 0;
   cluster_sync_all();
-  u64* lists = reinterpret_cast<u64*>(row_smem);  // [parts][k]: the row is no longer needed
+  u64* lists = reinterpret_cast<u64*>(row_smem) + list_offset;  // [parts][k] behind the row
   for (int q = tid; q < parts * k; q += DT) {
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];"
@@ -560,7 +612,8 @@ __device__ __forceinline__ int load_index(const void* p, int wide, long long i, 
   return v >= 0 && v < n ? static_cast<int>(v) : -1;
 }
 
-constexpr int FT = 256;  // threads of the forward and backward kernels
+constexpr int FT = 256;       // threads of the forward and backward kernels
+constexpr int ENTRIES = 128;  // kept classes whose logits stay in shared memory
 
 struct DistillParams {
   const void* values;
@@ -604,11 +657,10 @@ struct Running {
 
 // The student's exponentials are summed over the classes that are NOT kept: the kept ones are taken
 // out of the row in shared memory (each entry writes its number over its class, one that finds
-// another's number there is listed twice; then -inf replaces the numbers). Every thread takes the
-// maximum of its own vectors and sums relative to it. The at most k + 1 terms of the divergence are
-// evaluated in 64 bits: where student and teacher agree their first-order parts cancel, and so do
-// q - p in the gradient. stats and slopes leave nothing but one exponential per class to the
-// backward pass.
+// another's number there is listed twice; then -inf replaces the numbers). Two passes over the row,
+// maximum and sum, then one warp evaluates the at most k + 1 terms of the divergence in 64 bits:
+// where student and teacher agree their first-order parts cancel, and so do q - p in the gradient.
+// stats and slopes leave nothing but one exponential per class to the backward pass.
 template <typename T>
 __global__ void __launch_bounds__(FT)
 distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
@@ -617,9 +669,11 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   using Ord = Order<T>;
   using Tag = typename std::conditional<sizeof(T) == 4, uint32_t, unsigned short>::type;
   extern __shared__ __align__(16) uint4 row_smem[];
-  __shared__ double red_d[DW];
-  __shared__ float4 red_run[DW];
-  __shared__ float4 part_run[MAX_PARTS];
+  __shared__ int ent_at[ENTRIES];
+  __shared__ double ent_t[ENTRIES], ent_z[ENTRIES], ent_et[ENTRIES], ent_ez[ENTRIES];
+  __shared__ uint32_t red_u[DW];
+  __shared__ float red_f[DW];
+  __shared__ __align__(16) float4 part_run[MAX_PARTS];
   __shared__ __align__(8) uint64_t bar_mem;
   __shared__ int repeated, gave_up;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -630,85 +684,91 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   const uint32_t bar = smem_u32(&bar_mem);
   const StagedRow<T, DT> st(x, n, part, p.parts, row_smem, bar);
   if (tid == 0) repeated = gave_up = 0;
-  // The first DT entries stay in registers: class, teacher's logit, student's logit.
+  // The first ENTRIES entries stay in shared memory: class, teacher's logit, student's logit.
   const double inv_t = 1.0 / p.temperature;
-  int my_at = -1;
-  double my_t = -INFINITY, my_z = -INFINITY;
-  if (tid < k) {
-    my_at = load_index(p.indices, p.indices_wide, r * p.ld_indices + tid, n);
-    my_t = load_value(p.values, p.values_dtype, r * p.ld_values + tid) * inv_t;
-    if (my_at >= 0) my_z = to_float(x[my_at]) * inv_t;
+  auto load_entry = [&](int i, double& t, double& z) {
+    const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+    t = z = -INFINITY;
+    if (at >= 0) {
+      t = load_value(p.values, p.values_dtype, r * p.ld_values + i) * inv_t;
+      z = to_float(x[at]) * inv_t;
+    }
+    return at;
+  };
+  if (tid < min(k, ENTRIES)) {
+    double t, z;
+    ent_at[tid] = load_entry(tid, t, z);
+    ent_t[tid] = t;
+    ent_z[tid] = z;
   }
   const float c = p.c;
-  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
   __syncthreads();
   if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
   auto class_at = [&](int i) {
-    return i == tid ? my_at : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+    return i < ENTRIES ? ent_at[i] : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
   };
   Tag* tags = reinterpret_cast<Tag*>(row_smem);
   const int base = st.v0 * W - st.off, span = (st.v1 - st.v0) * W;
+  auto here = [&](int i) {  // place in this part of the row, -1: none
+    const int at = class_at(i);
+    return at >= 0 && at >= base && at - base < span ? at - base : -1;
+  };
   for (int i = tid; i < k; i += DT) {
-    const int at = class_at(i) - base;
-    if (class_at(i) >= 0 && at >= 0 && at < span) tags[at] = static_cast<Tag>(i);
+    const int at = here(i);
+    if (at >= 0) tags[at] = static_cast<Tag>(i);
   }
   __syncthreads();
   for (int i = tid; i < k; i += DT) {
-    const int at = class_at(i) - base;
-    if (class_at(i) >= 0 && at >= 0 && at < span && tags[at] != static_cast<Tag>(i)) repeated = 1;
+    const int at = here(i);
+    if (at >= 0 && tags[at] != static_cast<Tag>(i)) repeated = 1;
   }
   __syncthreads();
   for (int i = tid; i < k; i += DT) {
-    const int at = class_at(i) - base;
-    if (class_at(i) >= 0 && at >= 0 && at < span) reinterpret_cast<T*>(row_smem)[at] = from_float<T>(-INFINITY);
+    const int at = here(i);
+    if (at >= 0) reinterpret_cast<T*>(row_smem)[at] = from_float<T>(-INFINITY);
   }
   __syncthreads();
 
-  Running run = {-INFINITY, INFINITY, 0.0f};
+  // Largest value of the part, then the sum relative to it.
   const int nv = st.v1 - st.v0;
-  {
-    uint32_t m0 = Ord::kLow, m1 = Ord::kLow;
-    int i = tid;
-    for (; i + DT < nv; i += 2 * DT) {
-      m0 = Ord::largest(m0, st.row[i]);
-      m1 = Ord::largest(m1, st.row[i + DT]);
-    }
-    if (i < nv) m0 = Ord::largest(m0, st.row[i]);
-    const uint32_t best = max(Ord::key_of_largest(m0), Ord::key_of_largest(m1));
-    const float top = Ord::value(best);
-    run.m = top;  // NaN: the sum below is NaN
-    run.a = -top * c;
-    if (run.far()) {
-      if (top != -INFINITY) {
-        for (int j = tid; j < nv; j += DT) {
-          float v[W];
-          unpack(st.row[j], v, T());
-#pragma unroll
-          for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - top) * c);
-        }
-      }
-      if (top != top) run.m = 0.0f, run.a = 0.0f;
-    } else {
-      f32x2 acc = f2_pack(0.0f, 0.0f);
-#pragma unroll 2
-      for (int j = tid; j < nv; j += DT) add_exponentials<T>(st.row[j], c, run.a, acc);
-      float s0, s1;
-      f2_unpack(acc, s0, s1);
-      run.s = s0 + s1;
-    }
+  uint32_t m0 = Ord::kLow, m1 = Ord::kLow;
+  int i0 = tid;
+  for (; i0 + DT < nv; i0 += 2 * DT) {
+    m0 = Ord::largest(m0, st.row[i0]);
+    m1 = Ord::largest(m1, st.row[i0 + DT]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, run.m, o);
-    const float a = __shfl_xor_sync(0xffffffffu, run.a, o);
-    const float s = __shfl_xor_sync(0xffffffffu, run.s, o);
-    run.join(m, a, s, c);
-  }
-  if (lane == 0) red_run[warp] = make_float4(run.m, run.a, run.s, 0.0f);
+  if (i0 < nv) m0 = Ord::largest(m0, st.row[i0]);
+  uint32_t best = __reduce_max_sync(0xffffffffu, max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)));
+  if (lane == 0) red_u[warp] = best;
   __syncthreads();
-  run = {red_run[0].x, red_run[0].y, red_run[0].z};
 #pragma unroll
-  for (int i = 1; i < DW; ++i) run.join(red_run[i].x, red_run[i].y, red_run[i].z, c);
+  for (int i = 0; i < DW; ++i) best = max(best, red_u[i]);
+  const float top = Ord::value(best);
+  Running run = {top, -top * c, 0.0f};
+  if (!run.far()) {
+    f32x2 acc = 0;
+#pragma unroll 2
+    for (int j = tid; j < nv; j += DT) acc = f2_add(acc, exponentials<T>(st.row[j], c, run.a));
+    float s0, s1;
+    f2_unpack(acc, s0, s1);
+    run.s = s0 + s1;
+  } else if (top != -INFINITY) {  // NaN and +inf make the sum NaN
+    for (int j = tid; j < nv; j += DT) {
+      float v[W];
+      unpack(st.row[j], v, T());
+#pragma unroll
+      for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - top) * c);
+    }
+    if (top != top) run.m = run.a = 0.0f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
+  if (lane == 0) red_f[warp] = run.s;
+  __syncthreads();
+  if (warp != 0 && p.parts == 1) return;  // one warp finishes the row
+  run.s = red_f[0];
+#pragma unroll
+  for (int i = 1; i < DW; ++i) run.s += red_f[i];
   if (p.parts > 1) {
     if (tid == 0) {
       const uint32_t dst = mapa_shared(smem_u32(part_run + part), 0);
@@ -718,20 +778,21 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
                    : "memory");
     }
     cluster_sync_all();
-    if (part != 0) return;
+    if (part != 0 || warp != 0) return;
     run = {part_run[0].x, part_run[0].y, part_run[0].z};
     int any = __float_as_int(part_run[0].w);
     for (int i = 1; i < p.parts; ++i) {
       run.join(part_run[i].x, part_run[i].y, part_run[i].z, c);
       any |= __float_as_int(part_run[i].w);
     }
-    if (tid == 0) repeated = any & 1, gave_up = any >> 1;
-    __syncthreads();
+    if (lane == 0) repeated = any & 1, gave_up = any >> 1;
+    __syncwarp();
   }
 
   // Natural-log units from here on, in 64 bits, maxima and sums kept apart (a maximum of the size
   // of a mask's value would swallow the logarithm of its sum). zm, zs: the classes not kept;
   // fmaf(m, c, a) is what rounding the anchor to fp32 left over.
+  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
   const bool some = run.s != 0.0f;
   const double zm = some ? run.m * inv_t : -INFINITY;
   const double zs = run.far() ? run.s : run.s * exp2(-static_cast<double>(fmaf(run.m, c, run.a)));
@@ -740,60 +801,78 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     if (at < 0) return false;
     if (repeated)  // the first entry of a class counts
       for (int j = 0; j < i; ++j)
-        if (load_index(p.indices, p.indices_wide, r * p.ld_indices + j, n) == at) return false;
-    if (i == tid) {
-      t = my_t;
-      z = my_z;
+        if (class_at(j) == at) return false;
+    if (i < ENTRIES) {
+      t = ent_t[i];
+      z = ent_z[i];
     } else {
-      t = load_value(p.values, p.values_dtype, r * p.ld_values + i) * inv_t;
-      z = to_float(x[at]) * inv_t;
+      load_entry(i, t, z);
     }
     return true;
   };
+  auto warp_max = [](double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = Max()(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  auto warp_sum = [](double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
   double t_max = tr, z_max = zm;
-  for (int i = tid; i < k; i += DT) {
+  for (int i = lane; i < k; i += 32) {
     double t, z;
     if (!entry(i, t, z)) continue;
     t_max = Max()(t, t_max);
     z_max = Max()(z, z_max);
   }
-  t_max = block_reduce<DT>(t_max, red_d, Max());
-  z_max = block_reduce<DT>(z_max, red_d, Max());
-  auto part_of = [](double v, double top) { return v == -INFINITY ? 0.0 : exp(v - top); };
+  t_max = warp_max(t_max);
+  z_max = warp_max(z_max);
+  // Probabilities up to their common factor, kept in place of the logits' exponentials.
+  auto part_of = [](double v, double top_value) { return v == -INFINITY ? 0.0 : exp(v - top_value); };
   double t_sum = 0.0, z_sum = 0.0;
-  for (int i = tid; i < k; i += DT) {
+  for (int i = lane; i < k; i += 32) {
     double t, z;
     if (!entry(i, t, z)) continue;
-    t_sum += part_of(t, t_max);
-    z_sum += part_of(z, z_max);
+    const double et = part_of(t, t_max), ez = part_of(z, z_max);
+    t_sum += et;
+    z_sum += ez;
+    if (i < ENTRIES) {
+      ent_et[i] = et;
+      ent_ez[i] = ez;
+    }
   }
-  t_sum = block_reduce<DT>(t_sum, red_d, Sum()) + part_of(tr, t_max);
-  z_sum = block_reduce<DT>(z_sum, red_d, Sum()) + part_of(zm, z_max) * zs;
-  const double t_log = log(t_sum), z_log = log(z_sum);
+  const double e_tr = part_of(tr, t_max), e_zr = part_of(zm, z_max) * zs;
+  t_sum = warp_sum(t_sum) + e_tr;
+  z_sum = warp_sum(z_sum) + e_zr;
+  const double t_log = log(t_sum), z_log = log(z_sum), t_inv = 1.0 / t_sum, z_inv = 1.0 / z_sum;
   // Teacher's and student's probability of an outcome, and its term of the divergence. A teacher
   // without any mass (no entry left, no rest) teaches nothing.
   const bool silent = t_max == -INFINITY;
   double loss = 0.0;
-  auto outcome = [&](double t, double z, double sum, double& q) {  // student: sum * e^z
-    const double pt = t == -INFINITY ? 0.0 : exp(t - t_max - t_log);
-    const double log_q = z == -INFINITY ? z : z - z_max + log(sum) - z_log;
-    q = silent ? 0.0 : exp(log_q);
-    if (pt != 0.0) loss += pt * ((t - t_max - t_log) - log_q);
+  auto outcome = [&](double t, double et, double z, double ez, double z_extra, double& q) {
+    const double pt = t == -INFINITY ? 0.0 : et * t_inv;
+    q = silent || z == -INFINITY ? 0.0 : ez * z_inv;
+    if (pt != 0.0)
+      loss += pt * ((t - t_max - t_log) - (z == -INFINITY ? z : z - z_max + z_extra - z_log));
     return pt;
   };
-  for (int i = tid; i < k; i += DT) {
+  for (int i = lane; i < k; i += 32) {
     double t, z, q;
     float slope = 0.0f;
     if (entry(i, t, z)) {
-      const double pt = outcome(t, z, 1.0, q);
+      const double et = i < ENTRIES ? ent_et[i] : part_of(t, t_max);
+      const double ez = i < ENTRIES ? ent_ez[i] : part_of(z, z_max);
+      const double pt = outcome(t, et, z, ez, 0.0, q);
       slope = static_cast<float>(q - pt);
     }
     p.slopes[r * k + i] = slope;
   }
   double q_rest = 0.0, p_rest = 0.0;
-  if (tid == 0) p_rest = outcome(tr, zm, zs, q_rest);
-  loss = block_reduce<DT>(loss, red_d, Sum());
-  if (tid == 0) {
+  if (lane == 0) p_rest = outcome(tr, e_tr, zm, e_zr, log(zs), q_rest);
+  loss = warp_sum(loss);
+  if (lane == 0) {
     p.loss[r] = gave_up ? NAN : static_cast<float>(loss * p.temperature * p.temperature);
     // Gradient of a class that is not kept: q_j (1 - p_rest / q_rest).
     p.stats[r] = make_float2(run.m, some ? static_cast<float>((q_rest - p_rest) / run.s) : 0.0f);
@@ -889,7 +968,7 @@ int launch_clusters(void (*kernel)(Params...), int64_t rows, int parts, int thre
   if (smem > 24 * 1024) {  // may pass the default limit together with the static part
     const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               MAX_PART_BYTES + 64);
+                                               MAX_PART_BYTES + MAX_PARTS * 256 * 8);
     if (e != cudaSuccess) {
       set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
       cudaGetLastError();
@@ -950,7 +1029,8 @@ int top_logits(const void* logits, int64_t rows, int64_t n, int64_t ld, int64_t 
                void* values, int32_t* indices, float* rest, cudaStream_t stream) {
   size_t smem = 0;
   const int parts = staged_parts(rows, n, sizeof(T), 256, &smem);
-  if (parts > 1 && smem < static_cast<size_t>(parts * k * 8)) smem = static_cast<size_t>(parts * k * 8);
+  const int list_offset = static_cast<int>(smem / 8);
+  if (parts > 1) smem += static_cast<size_t>(parts * k * 8);
   const float c = static_cast<float>(1.4426950408889634 / temperature);
   const double inv_t = 1.0 / temperature;
   // More threads give more maxima to bound the k-th largest value with.
@@ -958,7 +1038,7 @@ int top_logits(const void* logits, int64_t rows, int64_t n, int64_t ld, int64_t 
   auto kernel = threads == 512 ? top_logits_kernel<T, 512> : top_logits_kernel<T, 256>;
   return launch_clusters(kernel, rows, parts, threads, smem, stream, static_cast<const T*>(logits),
                          static_cast<long long>(ld), static_cast<int>(n), static_cast<int>(k), c, inv_t,
-                         parts, static_cast<T*>(values), indices, rest);
+                         parts, list_offset, static_cast<T*>(values), indices, rest);
 }
 
 }  // namespace
