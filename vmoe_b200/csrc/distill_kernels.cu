@@ -27,6 +27,7 @@ void set_error(const char* fmt, const char* a, int code);
 namespace {
 
 constexpr int MAX_PARTS = 8;  // CTAs that can share a row (portable cluster size)
+constexpr int MAX_PART_BYTES = 176 * 1024;  // of a row in one CTA's shared memory
 
 typedef unsigned long long u64;
 
@@ -119,6 +120,7 @@ struct Order<float> {
   }
   static constexpr uint32_t kLow = 0xff800000u;  // -inf, as `largest` starts
   static __device__ __forceinline__ uint32_t key_of_largest(uint32_t m) { return key(m); }
+  static __device__ __forceinline__ float value_of_largest(uint32_t m) { return __uint_as_float(m); }
   static __device__ __forceinline__ bool all_below(uint32_t m, float bound) {
     return __uint_as_float(m) < bound;
   }
@@ -152,6 +154,11 @@ struct Order16 {
   static __device__ __forceinline__ uint32_t key_of_largest(uint32_t m) {
     const uint32_t a = key(m & 0xffffu), b = key(m >> 16);
     return a > b ? a : b;
+  }
+  static __device__ __forceinline__ float value_of_largest(uint32_t m) {
+    const uint32_t one = max2(m, m >> 16);  // the larger half in the low 16 bits
+    const unsigned short h = static_cast<unsigned short>(one);
+    return to_float(*reinterpret_cast<const T*>(&h));
   }
   static __device__ __forceinline__ bool all_below(uint32_t m, float bound) {
     const unsigned short h0 = static_cast<unsigned short>(m), h1 = static_cast<unsigned short>(m >> 16);
@@ -283,7 +290,6 @@ struct StagedRow {
 };
 
 // ------------------------------------------------------------------------------- top logits
-constexpr int TOP_CAP = 1024;  // candidates that shared memory holds
 constexpr int TOP_K_MAX = 256;
 
 // The k largest of the threads' maxima (found by one warp's bisection on their order keys) bound the
@@ -302,6 +308,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
                   int parts, int list_offset, T* __restrict__ values, int* __restrict__ indices,
                   float* __restrict__ rest) {
   constexpr int W = Vec<T>::W;
+  constexpr int TOP_CAP = 2 * DT;  // candidates that shared memory holds
   using Ord = Order<T>;
   extern __shared__ __align__(16) uint4 row_smem[];
   __shared__ __align__(16) u64 cand[TOP_CAP];
@@ -350,18 +357,34 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     lo = __reduce_min_sync(0xffffffffu, lo);
     filled = __reduce_add_sync(0xffffffffu, filled);
     if (filled < mine || mine == 0) lo = hi = 0;
-    while (lo < hi) {  // count(>= lo) >= mine; the bound is <= hi
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      int got = 0;
+    // count(>= lo) >= mine, the bound is <= hi. Three counts per step, in one word: a quarter of the
+    // range is left for the time of one reduction.
+    while (lo < hi) {
+      const uint32_t step = (hi - lo) / 4;
+      const uint32_t m1 = lo + step + 1, m2 = m1 + step, m3 = min(m2 + step, hi);
+      uint32_t got = 0;
 #pragma unroll
-      for (int q = 0; q < DT / 32; ++q) got += own[q] >= mid ? 1 : 0;
+      for (int q = 0; q < DT / 32; ++q)
+        got += (own[q] >= m1 ? 1u : 0u) + (own[q] >= m2 ? 1u << 10 : 0u) + (own[q] >= m3 ? 1u << 20 : 0u);
       got = __reduce_add_sync(0xffffffffu, got);
-      if (got >= mine) {
-        lo = mid;
-        if (got <= mine + mine / 8 + 4) break;
+      const int g1 = got & 1023, g2 = (got >> 10) & 1023, g3 = got >> 20;
+      int g;
+      if (g3 >= mine) {
+        lo = m3;
+        g = g3;
+      } else if (g2 >= mine) {
+        lo = m2;
+        hi = m3 - 1;
+        g = g2;
+      } else if (g1 >= mine) {
+        lo = m1;
+        hi = m2 - 1;
+        g = g1;
       } else {
-        hi = mid - 1;
+        hi = m1 - 1;
+        continue;
       }
+      if (g <= mine + mine / 8 + 4) break;
     }
     if (tid == 0) first_bound = lo;
   }
@@ -395,17 +418,26 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
         }
       }
     };
+    if (attempt == 0) {
+      u64 mine_hot = 0;  // bit i: vector tid + i DT (at most MAX_PART_BYTES / 16 / DT = 44 of them)
+      int j = tid;
 #pragma unroll 2
-    for (int j = tid; j < nv; j += DT) {
-      const uint4 q = st.row[j];
-      const f32x2 sum = exponentials<T>(q, c, anchor);
-      if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) {
-        acc = f2_add(acc, sum);
-      } else if (attempt == 0) {
-        const int pos = atomicAdd(&hot_count, 1);
-        if (pos < TOP_CAP) hot[pos] = j;
-      } else {  // exact bounds: any number of vectors may hold values equal to the bound
-        take_apart(j, q);
+      for (int i = 0; j < nv; j += DT, ++i) {
+        const uint4 q = st.row[j];
+        const f32x2 sum = exponentials<T>(q, c, anchor);
+        if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) acc = f2_add(acc, sum);
+        else mine_hot |= 1ull << i;
+      }
+      if (mine_hot) {
+        int pos = atomicAdd(&hot_count, __popcll(mine_hot));
+        for (; mine_hot && pos < TOP_CAP; mine_hot &= mine_hot - 1, ++pos)
+          hot[pos] = tid + (__ffsll(mine_hot) - 1) * DT;
+      }
+    } else {  // exact bounds: any number of vectors may hold values equal to the bound
+      for (int j = tid; j < nv; j += DT) {
+        const uint4 q = st.row[j];
+        if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) acc = f2_add(acc, exponentials<T>(q, c, anchor));
+        else take_apart(j, q);
       }
     }
     __syncthreads();
@@ -459,19 +491,23 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   }
   const int found = min(count, TOP_CAP);  // >= mine
 
-  // Rank of every candidate = number of larger ones (all are different: the position is part).
-  if (tid == 0 && (found & 1)) cand[found] = 0;  // found < TOP_CAP then; read in pairs below
+  // Rank of every candidate = number of larger ones (all are different: the position is part). Four
+  // threads count for one candidate.
+  if (tid < 8 && found + tid < TOP_CAP) cand[found + tid] = 0;  // the list is read in blocks of 8
   __syncthreads();
-  for (int q = tid; q < found; q += DT) {
-    const u64 me = cand[q];
+  for (int q0 = 0; q0 < found; q0 += DT / 4) {
+    const int q = q0 + (tid >> 2);
+    const u64 me = q < found ? cand[q] : ~0ull;
     int rank = 0;
     const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
-#pragma unroll 4
-    for (int j = 0; j < (found + 1) / 2; ++j) {
+#pragma unroll 2
+    for (int j = tid & 3; j < (found + 1) / 2; j += 4) {
       const ulonglong2 two = pairs[j];
       rank += (two.x > me ? 1 : 0) + (two.y > me ? 1 : 0);
     }
-    sorted[rank] = me;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (q < found && (tid & 3) == 0) sorted[rank] = me;
   }
   s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
   if (fabsf(m) < FAR)  // the last factor takes the rounding of m c back
@@ -657,9 +693,10 @@ struct Running {
 
 // The student's exponentials are summed over the classes that are NOT kept: the kept ones are taken
 // out of the row in shared memory (each entry writes its number over its class, one that finds
-// another's number there is listed twice; then -inf replaces the numbers). Two passes over the row,
-// maximum and sum, then one warp evaluates the at most k + 1 terms of the divergence in 64 bits:
-// where student and teacher agree their first-order parts cancel, and so do q - p in the gradient.
+// another's number there is listed twice; then -inf replaces the numbers). One pass sums relative to
+// the largest value met. One warp evaluates the at most k + 1 terms of the divergence in 64 bits,
+// where the parts that cancel between a student and a teacher that agree do no harm, nor in the
+// gradient's q - p: all but the student's normaliser while the row is still on its way.
 // stats and slopes leave nothing but one exponential per class to the backward pass.
 template <typename T>
 __global__ void __launch_bounds__(FT)
@@ -671,9 +708,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   extern __shared__ __align__(16) uint4 row_smem[];
   __shared__ int ent_at[ENTRIES];
   __shared__ double ent_t[ENTRIES], ent_z[ENTRIES], ent_et[ENTRIES], ent_ez[ENTRIES];
-  __shared__ uint32_t red_u[DW];
-  __shared__ float red_f[DW];
-  __shared__ __align__(16) float4 part_run[MAX_PARTS];
+  __shared__ __align__(16) float4 red_run[DW], part_run[MAX_PARTS];
   __shared__ __align__(8) uint64_t bar_mem;
   __shared__ int repeated, gave_up;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -684,7 +719,8 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   const uint32_t bar = smem_u32(&bar_mem);
   const StagedRow<T, DT> st(x, n, part, p.parts, row_smem, bar);
   if (tid == 0) repeated = gave_up = 0;
-  // The first ENTRIES entries stay in shared memory: class, teacher's logit, student's logit.
+  // While the row is on its way the first warp works on the kept entries: their classes, teacher's and
+  // student's logits, both sides' exponentials and sums. The first ENTRIES of them stay in shared memory.
   const double inv_t = 1.0 / p.temperature;
   auto load_entry = [&](int i, double& t, double& z) {
     const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
@@ -703,10 +739,82 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   }
   const float c = p.c;
   __syncthreads();
-  if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
   auto class_at = [&](int i) {
     return i < ENTRIES ? ent_at[i] : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
   };
+  auto warp_max = [](double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = Max()(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  auto warp_sum = [](double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  // Natural-log units in 64 bits, maxima and sums kept apart (a maximum of the size of a mask's value
+  // would swallow the logarithm of its sum). A class that is listed twice is sorted out later, with
+  // everything here done again.
+  const double tr = p.rest && warp == 0 ? static_cast<double>(p.rest[r]) : -INFINITY;
+  double t_max, z_max, t_sum, z_sum, t_inv, t_log, fixed_loss, mass;
+  bool silent;
+  auto part_of = [](double v, double top_value) { return v == -INFINITY ? 0.0 : exp(v - top_value); };
+  auto entry = [&](int i, double& t, double& z) {  // teacher's and student's logit; false: left out
+    const int at = class_at(i);
+    if (at < 0) return false;
+    if (repeated)  // the first entry of a class counts
+      for (int j = 0; j < i; ++j)
+        if (class_at(j) == at) return false;
+    if (i < ENTRIES) {
+      t = ent_t[i];
+      z = ent_z[i];
+    } else {
+      load_entry(i, t, z);
+    }
+    return true;
+  };
+  auto work_on_entries = [&]() {
+    t_max = tr, z_max = -INFINITY;
+    for (int i = lane; i < k; i += 32) {
+      double t, z;
+      if (!entry(i, t, z)) continue;
+      t_max = Max()(t, t_max);
+      z_max = Max()(z, z_max);
+    }
+    t_max = warp_max(t_max);
+    z_max = warp_max(z_max);
+    t_sum = z_sum = 0.0;
+    for (int i = lane; i < k; i += 32) {
+      double t, z;
+      if (!entry(i, t, z)) continue;
+      const double et = part_of(t, t_max), ez = part_of(z, z_max);
+      t_sum += et;
+      z_sum += ez;
+      if (i < ENTRIES) {
+        ent_et[i] = et;
+        ent_ez[i] = ez;
+      }
+    }
+    t_sum = warp_sum(t_sum) + part_of(tr, t_max);
+    z_sum = warp_sum(z_sum);
+    silent = t_max == -INFINITY;  // a teacher without any mass (no entry, no rest) teaches nothing
+    t_inv = silent ? 0.0 : 1.0 / t_sum;
+    t_log = log(t_sum);
+    // sum p (log p - (z - z_max)): the loss up to the student's normaliser, which every outcome shares.
+    fixed_loss = mass = 0.0;
+    for (int i = lane; i < k; i += 32) {
+      double t, z;
+      if (!entry(i, t, z)) continue;
+      const double pt = (i < ENTRIES ? ent_et[i] : part_of(t, t_max)) * t_inv;
+      if (pt == 0.0) continue;
+      fixed_loss += pt * ((t - t_max - t_log) - (z == -INFINITY ? z : z - z_max));
+      mass += pt;
+    }
+    fixed_loss = warp_sum(fixed_loss);
+    mass = warp_sum(mass);
+  };
+  if (warp == 0 && part == 0) work_on_entries();
+  if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
   Tag* tags = reinterpret_cast<Tag*>(row_smem);
   const int base = st.v0 * W - st.off, span = (st.v1 - st.v0) * W;
   auto here = [&](int i) {  // place in this part of the row, -1: none
@@ -729,46 +837,67 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
   }
   __syncthreads();
 
-  // Largest value of the part, then the sum relative to it.
+  // One pass: every thread sums relative to the largest value it has met.
   const int nv = st.v1 - st.v0;
-  uint32_t m0 = Ord::kLow, m1 = Ord::kLow;
-  int i0 = tid;
-  for (; i0 + DT < nv; i0 += 2 * DT) {
-    m0 = Ord::largest(m0, st.row[i0]);
-    m1 = Ord::largest(m1, st.row[i0 + DT]);
-  }
-  if (i0 < nv) m0 = Ord::largest(m0, st.row[i0]);
-  uint32_t best = __reduce_max_sync(0xffffffffu, max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)));
-  if (lane == 0) red_u[warp] = best;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < DW; ++i) best = max(best, red_u[i]);
-  const float top = Ord::value(best);
-  Running run = {top, -top * c, 0.0f};
-  if (!run.far()) {
+  Running run = {-INFINITY, INFINITY, 0.0f};
+  {
     f32x2 acc = 0;
 #pragma unroll 2
-    for (int j = tid; j < nv; j += DT) acc = f2_add(acc, exponentials<T>(st.row[j], c, run.a));
+    for (int j = tid; j < nv; j += DT) {
+      const uint4 q = st.row[j];
+      const float top = Ord::value_of_largest(Ord::largest(Ord::kLow, q));
+      if (!(top <= run.m)) {  // NaN too
+        if (!(fabsf(top) < FAR) || run.far()) {
+          // Beginning, infinities, NaN, masks' values: one element at a time.
+          float s0, s1;
+          f2_unpack(acc, s0, s1);
+          run.s += s0 + s1;
+          acc = 0;
+          run.raise(top, c);
+          if (!run.far()) {
+            acc = exponentials<T>(q, c, run.a);
+          } else if (top != -INFINITY) {
+            float v[W];
+            unpack(q, v, T());
+#pragma unroll
+            for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
+          }
+          continue;
+        }
+        const float b = -top * c;
+        const float f = exp2_approx(b - run.a);
+        acc = f2_mul(acc, f2_pack(f, f));
+        run.s *= f;
+        run.m = top;
+        run.a = b;
+      } else if (run.far()) {
+        if (run.m > -INFINITY) {
+          float v[W];
+          unpack(q, v, T());
+#pragma unroll
+          for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
+        }
+        continue;
+      }
+      acc = f2_add(acc, exponentials<T>(q, c, run.a));
+    }
     float s0, s1;
     f2_unpack(acc, s0, s1);
-    run.s = s0 + s1;
-  } else if (top != -INFINITY) {  // NaN and +inf make the sum NaN
-    for (int j = tid; j < nv; j += DT) {
-      float v[W];
-      unpack(st.row[j], v, T());
-#pragma unroll
-      for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - top) * c);
-    }
-    if (top != top) run.m = run.a = 0.0f;
+    run.s += s0 + s1;
   }
+  {
+    uint32_t best = __reduce_max_sync(0xffffffffu, Order<float>::key(__float_as_uint(run.m)));
+    const float m = Order<float>::value(best);
+    if (m > run.m) run.raise(m, c);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
-  if (lane == 0) red_f[warp] = run.s;
+    for (int o = 16; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
+    if (lane == 0) red_run[warp] = make_float4(run.m, run.a, run.s, 0.0f);
+  }
   __syncthreads();
   if (warp != 0 && p.parts == 1) return;  // one warp finishes the row
-  run.s = red_f[0];
+  run = {red_run[0].x, red_run[0].y, red_run[0].z};
 #pragma unroll
-  for (int i = 1; i < DW; ++i) run.s += red_f[i];
+  for (int i = 1; i < DW; ++i) run.join(red_run[i].x, red_run[i].y, red_run[i].z, c);
   if (p.parts > 1) {
     if (tid == 0) {
       const uint32_t dst = mapa_shared(smem_u32(part_run + part), 0);
@@ -789,90 +918,33 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     __syncwarp();
   }
 
-  // Natural-log units from here on, in 64 bits, maxima and sums kept apart (a maximum of the size
-  // of a mask's value would swallow the logarithm of its sum). zm, zs: the classes not kept;
-  // fmaf(m, c, a) is what rounding the anchor to fp32 left over.
-  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
+  if (repeated) work_on_entries();  // without the entries of classes listed before
+  // The classes not kept: zs * e^zm; fmaf(m, c, a) is what rounding the anchor to fp32 left over.
   const bool some = run.s != 0.0f;
   const double zm = some ? run.m * inv_t : -INFINITY;
   const double zs = run.far() ? run.s : run.s * exp2(-static_cast<double>(fmaf(run.m, c, run.a)));
-  auto entry = [&](int i, double& t, double& z) {  // teacher's and student's logit; false: left out
-    const int at = class_at(i);
-    if (at < 0) return false;
-    if (repeated)  // the first entry of a class counts
-      for (int j = 0; j < i; ++j)
-        if (class_at(j) == at) return false;
-    if (i < ENTRIES) {
-      t = ent_t[i];
-      z = ent_z[i];
-    } else {
-      load_entry(i, t, z);
-    }
-    return true;
-  };
-  auto warp_max = [](double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = Max()(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-  };
-  auto warp_sum = [](double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
-  double t_max = tr, z_max = zm;
+  // The student's normaliser relative to z_max, through whichever maximum is larger.
+  const double top = Max()(zm, z_max);
+  const double e_zm = part_of(zm, top) * zs, e_zk = part_of(z_max, top);
+  const double total = z_sum * e_zk + e_zm, log_total = log(total);
+  const double z_log = top - z_max + log_total;  // only used with kept classes of finite logits
+  const double z_inv = e_zk / total;
   for (int i = lane; i < k; i += 32) {
     double t, z;
-    if (!entry(i, t, z)) continue;
-    t_max = Max()(t, t_max);
-    z_max = Max()(z, z_max);
-  }
-  t_max = warp_max(t_max);
-  z_max = warp_max(z_max);
-  // Probabilities up to their common factor, kept in place of the logits' exponentials.
-  auto part_of = [](double v, double top_value) { return v == -INFINITY ? 0.0 : exp(v - top_value); };
-  double t_sum = 0.0, z_sum = 0.0;
-  for (int i = lane; i < k; i += 32) {
-    double t, z;
-    if (!entry(i, t, z)) continue;
-    const double et = part_of(t, t_max), ez = part_of(z, z_max);
-    t_sum += et;
-    z_sum += ez;
-    if (i < ENTRIES) {
-      ent_et[i] = et;
-      ent_ez[i] = ez;
-    }
-  }
-  const double e_tr = part_of(tr, t_max), e_zr = part_of(zm, z_max) * zs;
-  t_sum = warp_sum(t_sum) + e_tr;
-  z_sum = warp_sum(z_sum) + e_zr;
-  const double t_log = log(t_sum), z_log = log(z_sum), t_inv = 1.0 / t_sum, z_inv = 1.0 / z_sum;
-  // Teacher's and student's probability of an outcome, and its term of the divergence. A teacher
-  // without any mass (no entry left, no rest) teaches nothing.
-  const bool silent = t_max == -INFINITY;
-  double loss = 0.0;
-  auto outcome = [&](double t, double et, double z, double ez, double z_extra, double& q) {
-    const double pt = t == -INFINITY ? 0.0 : et * t_inv;
-    q = silent || z == -INFINITY ? 0.0 : ez * z_inv;
-    if (pt != 0.0)
-      loss += pt * ((t - t_max - t_log) - (z == -INFINITY ? z : z - z_max + z_extra - z_log));
-    return pt;
-  };
-  for (int i = lane; i < k; i += 32) {
-    double t, z, q;
     float slope = 0.0f;
-    if (entry(i, t, z)) {
+    if (entry(i, t, z) && !silent) {
       const double et = i < ENTRIES ? ent_et[i] : part_of(t, t_max);
       const double ez = i < ENTRIES ? ent_ez[i] : part_of(z, z_max);
-      const double pt = outcome(t, et, z, ez, 0.0, q);
-      slope = static_cast<float>(q - pt);
+      slope = static_cast<float>((ez == 0.0 ? 0.0 : ez * z_inv) - et * t_inv);
     }
     p.slopes[r * k + i] = slope;
   }
-  double q_rest = 0.0, p_rest = 0.0;
-  if (lane == 0) p_rest = outcome(tr, e_tr, zm, e_zr, log(zs), q_rest);
-  loss = warp_sum(loss);
   if (lane == 0) {
+    double loss = mass > 0.0 || mass != mass ? fixed_loss + mass * (z_max == -INFINITY ? 0.0 : z_log) : 0.0;
+    const double p_rest = tr == -INFINITY ? 0.0 : part_of(tr, t_max) * t_inv;
+    const double q_rest = silent || !some ? 0.0 : e_zm / total;
+    if (p_rest != 0.0)
+      loss += p_rest * ((tr - t_max - t_log) - (some ? zm - top + log(zs) - log_total : -INFINITY));
     p.loss[r] = gave_up ? NAN : static_cast<float>(loss * p.temperature * p.temperature);
     // Gradient of a class that is not kept: q_j (1 - p_rest / q_rest).
     p.stats[r] = make_float2(run.m, some ? static_cast<float>((q_rest - p_rest) / run.s) : 0.0f);
@@ -959,8 +1031,6 @@ int check_launch() {
   }
   return 0;
 }
-
-constexpr int MAX_PART_BYTES = 176 * 1024;  // of a row in one CTA's shared memory
 
 template <typename... Params, typename... Args>
 int launch_clusters(void (*kernel)(Params...), int64_t rows, int parts, int threads, size_t smem,
