@@ -74,14 +74,6 @@ __device__ __forceinline__ void tma_store_4d(const void* desc, uint32_t src, int
       : "memory");
 }
 
-struct GatedParams {
-  const float* bias;  // forward: (E, 2, M) or NULL
-  float* sums;        // backward: (E, row blocks of 32, 2, M) partial column sums or NULL
-  int rows, k, m, batch;
-  int act;            // 0 GELU (tanh form), 1 SiLU
-  int save;           // forward: write a and s
-};
-
 // act(g) and act'(g) through one sigmoid: act = g sigma(w), act' = sigma (1 + g (1 - sigma) w').
 // GELU's tanh form is w = 2 sqrt(2/pi) (g + 0.044715 g^3), SiLU is w = g.
 __device__ __forceinline__ void gate_and_slope(float g, int act, float& a, float& slope) {
@@ -101,6 +93,25 @@ __device__ __forceinline__ void gate_and_slope(float g, int act, float& a, float
   a = g * sg;
   slope = sg * fmaf(g * (1.0f - sg), dw, 1.0f);
 }
+
+struct GatedParams {
+  const void* bias;   // forward: (E, 2, M) or NULL
+  const __nv_bfloat16* bias_out;  // forward: converted to fp32 for the GEMM behind, or NULL
+  float* bias_out_f32;
+  int bias_out_count, bias_bf16;
+  float* sums;        // backward: (E, row blocks of 32, 2, M) partial column sums or NULL
+  int rows, k, m, batch;
+  int act;            // 0 GELU (tanh form), 1 SiLU
+  int save;           // forward: write a and s
+};
+
+}  // namespace
+}  // namespace vmoe
+
+#include "gated_rows.cuh"
+
+namespace vmoe {
+namespace {
 
 // MODE 0: forward. A = x (rows x k), B = w_in as (k, m, 2 E), both K-major.
 // MODE 1: backward. A = dy (rows x k, K-major), B = w_out (m contiguous: MN-major).
@@ -298,6 +309,10 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     uint32_t in_phase = 0;
     int local = 0;
     bool ok = true;
+    if (MODE == 0 && p.bias_out)  // the GEMM behind this kernel takes fp32 biases
+      for (int i = static_cast<int>(blockIdx.x) * 32 * EPI_WARPS + 32 * ew + lane; i < p.bias_out_count;
+           i += static_cast<int>(gridDim.x) * 32 * EPI_WARPS)
+        p.bias_out_f32[i] = __bfloat162float(p.bias_out[i]);
     // One row of a chunk (32 packed values) into a staging tile.
     auto stage_row = [&](uint8_t* tile, const uint32_t (&w)[16]) {
 #pragma unroll
@@ -338,8 +353,26 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           tmem_ld_32x32(acc, rg);
           tmem_ld_32x32(acc + HALF, ru);
           tmem_ld_wait();
-          if (p.bias) {
-            const float* bg = p.bias + (2ll * b) * p.m + col0;
+          if (p.bias && p.bias_bf16) {
+            const __nv_bfloat16* bg = static_cast<const __nv_bfloat16*>(p.bias) + (2ll * b) * p.m + col0;
+            const __nv_bfloat16* bu = bg + p.m;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (col0 + i >= p.m) break;  // m is a multiple of 8
+              const uint4 g8 = __ldg(reinterpret_cast<const uint4*>(bg + i));
+              const uint4 u8 = __ldg(reinterpret_cast<const uint4*>(bu + i));
+              const uint32_t gw[4] = {g8.x, g8.y, g8.z, g8.w}, uw[4] = {u8.x, u8.y, u8.z, u8.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float2 gf = unpack_bf16x2(gw[q]), uf = unpack_bf16x2(uw[q]);
+                rg[i + 2 * q] = __float_as_uint(__uint_as_float(rg[i + 2 * q]) + gf.x);
+                rg[i + 2 * q + 1] = __float_as_uint(__uint_as_float(rg[i + 2 * q + 1]) + gf.y);
+                ru[i + 2 * q] = __float_as_uint(__uint_as_float(ru[i + 2 * q]) + uf.x);
+                ru[i + 2 * q + 1] = __float_as_uint(__uint_as_float(ru[i + 2 * q + 1]) + uf.y);
+              }
+            }
+          } else if (p.bias) {
+            const float* bg = static_cast<const float*>(p.bias) + (2ll * b) * p.m + col0;
             const float* bu = bg + p.m;
             if (col0 + 32 <= p.m) {
 #pragma unroll
@@ -491,24 +524,113 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   }
 }
 
-// out[e][c] (+)= sum over the row blocks of sums[e][block][c], blocks in order within a thread
-// group and groups in order, so the result does not depend on scheduling.
+// One set of partial column sums: out (e, cols) (+)= sums (e, blocks, cols) over its blocks.
+struct SumsPart {
+  const float* sums;
+  void* out;
+  int blocks, cols, out_bf16, accumulate;
+};
+
+__device__ __forceinline__ void put(void* out, int is_bf16, int accumulate, long long i, float v) {
+  if (is_bf16) {
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16(v);
+  } else {
+    float* o = static_cast<float*>(out) + i;
+    *o = accumulate ? *o + v : v;
+  }
+}
+
+// Blocks in order within a warp and warps in order, so the result does not depend on scheduling.
 __global__ void __launch_bounds__(256)
-gated_join_sums_kernel(const float* __restrict__ sums, float* __restrict__ out, int blocks, int cols,
-                       int accumulate) {
+gated_join_sums_kernel(const SumsPart a, const SumsPart b) {
   __shared__ float part[8][32];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  const float* src = sums + static_cast<long long>(blockIdx.y) * blocks * cols;
+  const int a_tiles = (a.cols + 31) / 32;
+  const bool in_a = static_cast<int>(blockIdx.x) < a_tiles;
+  const SumsPart& p = in_a ? a : b;
+  const int c = (static_cast<int>(blockIdx.x) - (in_a ? 0 : a_tiles)) * 32 + lane;
+  const float* src = p.sums + static_cast<long long>(blockIdx.y) * p.blocks * p.cols;
   float s = 0.0f;
-  if (c < cols)
-    for (int i = group; i < blocks; i += 8) s += src[static_cast<long long>(i) * cols + c];
+  if (c < p.cols)
+    for (int i = group; i < p.blocks; i += 8) s += src[static_cast<long long>(i) * p.cols + c];
   part[group][lane] = s;
   __syncthreads();
-  if (group == 0 && c < cols) {
+  if (group == 0 && c < p.cols) {
     for (int i = 1; i < 8; ++i) s += part[i][lane];
-    float* dst = out + static_cast<long long>(blockIdx.y) * cols + c;
-    *dst = accumulate ? *dst + s : s;
+    put(p.out, p.out_bf16, p.accumulate, static_cast<long long>(blockIdx.y) * p.cols + c, s);
+  }
+}
+
+// sums (e, blocks, n) of x (e, rows, n) over blocks of ROW_BLOCK rows: 8 columns per lane, a warp
+// every eighth row, its loads all in flight together.
+constexpr int ROW_BLOCK = 128;
+__global__ void __launch_bounds__(256)
+gated_row_sums_kernel(const __nv_bfloat16* __restrict__ x, float* __restrict__ sums, int rows, int n) {
+  __shared__ float part[8][256 + 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.x * 256 + lane * 8;
+  const int r0 = blockIdx.y * ROW_BLOCK + warp;
+  const __nv_bfloat16* src = x + static_cast<long long>(blockIdx.z) * rows * n;
+  uint4 q[ROW_BLOCK / 8];
+#pragma unroll
+  for (int i = 0; i < ROW_BLOCK / 8; ++i) {
+    const int r = r0 + 8 * i;
+    q[i] = r < rows && col < n
+               ? __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(r) * n + col))
+               : make_uint4(0, 0, 0, 0);
+  }
+  float s[8] = {};
+#pragma unroll
+  for (int i = 0; i < ROW_BLOCK / 8; ++i) {
+    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(w[j]);
+      s[2 * j] += f.x;
+      s[2 * j + 1] += f.y;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = s[j];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < n) {
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) total += part[w][threadIdx.x];
+    sums[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * n + c] = total;
+  }
+}
+
+// out (count) (+)= sum of `pieces` partial results, in order.
+__global__ void __launch_bounds__(256)
+gated_join_pieces_kernel(const float* __restrict__ pieces, void* __restrict__ out, long long count,
+                         int n_pieces, int out_bf16, int accumulate) {
+  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= count) return;  // count is a multiple of 64
+  float4 s = __ldg(reinterpret_cast<const float4*>(pieces + i));
+  for (int p = 1; p < n_pieces; ++p) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(pieces + p * count + i));
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  if (out_bf16) {
+    uint2 q;
+    q.x = pack_bf16x2(s.x, s.y);
+    q.y = pack_bf16x2(s.z, s.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + i) = q;
+  } else {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i);
+    if (accumulate) {
+      const float4 v = *o;
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    *o = s;
   }
 }
 
@@ -612,13 +734,23 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh, 
   return 0;
 }
 
-int check_args(const VmoeGatedArgs* a) {
-  if (a->e < 0 || a->rows < 0 || a->k < 1 || a->m < 1) return fail("gated mlp: bad sizes");
-  if (a->rows > (1 << 28) || a->k > (1 << 24) || a->m > (1 << 24) || a->e > (1 << 20))
+int check_launch() {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+    return -5;
+  }
+  return 0;
+}
+
+int check_sizes(const VmoeGatedArgs* a) {
+  if (a->e < 0 || a->rows < 0 || a->h < 1 || a->m < 1 || a->o < 1) return fail("gated mlp: bad sizes");
+  if (a->rows > (1 << 28) || a->h > (1 << 24) || a->m > (1 << 24) || a->o > (1 << 24) || a->e > 32767)
     return fail("gated mlp: sizes out of range");
-  if (a->k % 8 || a->m % 8 || a->lda % 8 || a->a_batch_stride % 8)
+  if (a->h % 8 || a->m % 8 || a->o % 8 || a->ld_res % 8 || a->res_batch_stride % 8)
     return fail("gated mlp: widths and strides must be multiples of 8 elements");
-  const void* ptrs[6] = {a->a, a->w, a->hid, a->saved, a->grad, a->bias};
+  const void* ptrs[15] = {a->x,     a->w_in, a->w_out, a->b_in, a->b_out, a->residual, a->y,     a->hid,
+                          a->saved, a->dy,   a->dgu,   a->dx,   a->dw_in, a->dw_out,   a->scratch};
   for (const void* q : ptrs)
     if (reinterpret_cast<uintptr_t>(q) & 15) return fail("gated mlp: operands must be 16-byte aligned");
   if (a->act != 0 && a->act != 1) return fail("gated mlp: unknown activation");
@@ -631,24 +763,201 @@ bool use_pairs(const VmoeGatedArgs* a, const DeviceInfo& info, int tn) {
   return info.pairs > 0 && a->rows >= 2 * BM && tiles >= info.pairs / 2;
 }
 
+// The few-row kernel: rows of x in groups of 8.
+constexpr int FEW_ROWS = 16;
+
+template <int NT, bool GATED>
+int launch_rows(RowsParams p, int e, int sms, cudaStream_t stream) {
+  const int tiles = (p.m + 15) / 16, chunks = (p.k + 31) / 32;
+  // Share the contraction over a cluster until every SM has a CTA, while each warp keeps a chunk.
+  p.split = 1;
+  while (p.split < GR_MAX_SPLIT && tiles * e * p.split < sms && chunks >= 2 * p.split * GR_WARPS) p.split *= 2;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[2];
+  memset(attr, 0, sizeof(attr));
+  int n = 0;
+  if (p.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (p.after) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split), static_cast<unsigned>(e));
+  cfg.blockDim = dim3(GR_THREADS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, gated_rows_kernel<NT, GATED>, p);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s (code %d)", cudaGetErrorString(err), static_cast<int>(err));
+    return -5;
+  }
+  return 0;
+}
+
+int few_rows(const VmoeGatedArgs* a, const DeviceInfo& info, cudaStream_t stream) {
+  RowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = static_cast<const __nv_bfloat16*>(a->x);
+  p.w = static_cast<const __nv_bfloat16*>(a->w_in);
+  p.bias = a->b_in;
+  p.bias_bf16 = a->b_in_bf16;
+  p.out = static_cast<__nv_bfloat16*>(a->hid);
+  p.saved = static_cast<__nv_bfloat16*>(a->saved);
+  p.ldx = a->h;
+  p.x_batch_stride = a->rows * a->h;
+  p.rows = static_cast<int>(a->rows);
+  p.k = static_cast<int>(a->h);
+  p.m = static_cast<int>(a->m);
+  p.act = a->act;
+  const int e = static_cast<int>(a->e);
+  int rc = a->rows <= 8 ? launch_rows<1, true>(p, e, info.sms, stream)
+                        : launch_rows<2, true>(p, e, info.sms, stream);
+  if (rc) return rc;
+  RowsParams q;
+  memset(&q, 0, sizeof(q));
+  q.x = static_cast<const __nv_bfloat16*>(a->hid);
+  q.w = static_cast<const __nv_bfloat16*>(a->w_out);
+  q.bias = a->b_out;
+  q.bias_bf16 = a->b_out_bf16;
+  q.residual = static_cast<const __nv_bfloat16*>(a->residual);
+  q.out = static_cast<__nv_bfloat16*>(a->y);
+  q.ldx = a->m;
+  q.x_batch_stride = a->rows * a->m;
+  q.ldr = a->ld_res;
+  q.r_batch_stride = a->res_batch_stride;
+  q.rows = static_cast<int>(a->rows);
+  q.k = static_cast<int>(a->m);
+  q.m = static_cast<int>(a->o);
+  q.after = 1;
+  return a->rows <= 8 ? launch_rows<1, false>(q, e, info.sms, stream)
+                      : launch_rows<2, false>(q, e, info.sms, stream);
+}
+
+void gemm_operands(VmoeGemmArgs* g, const void* a, int64_t lda, int64_t sa, int a_mn, const void* b,
+                   int64_t ldb, int64_t sb, int b_mn, int64_t m, int64_t n, int64_t k, int64_t batch) {
+  memset(g, 0, sizeof(*g));
+  g->A = a;
+  g->B = b;
+  g->M = m;
+  g->N = n;
+  g->K = k;
+  g->batch = batch;
+  g->lda = lda;
+  g->ldb = ldb;
+  g->ldc = n;
+  g->a_batch_stride = batch > 1 ? sa : 0;
+  g->b_batch_stride = batch > 1 ? sb : 0;
+  g->c_batch_stride = batch > 1 ? m * n : 0;
+  g->a_mn_major = a_mn;
+  g->b_mn_major = b_mn;
+  g->split_k = 1;
+}
+
+// Pieces that a weight gradient's contraction over `rows` is cut into: few output tiles leave SMs
+// idle in the last round, each piece costs writing and reading its fp32 result once.
+int gradient_pieces(int64_t e, int64_t n, int64_t k, int64_t rows) {
+  const int64_t tiles = e * ((n + 255) / 256) * ((k + 255) / 256), pairs = 74;
+  if (e > 1 || tiles >= 2 * pairs || rows < 4096) return 1;
+  const double round_s = 2.0 * 256 * 256 * rows / (1.5e15 / pairs), piece_s = n * k * 8.0 / 5e12;
+  int best = 1;
+  double best_s = round_s * ((tiles + pairs - 1) / pairs);
+  for (int s = 2; s <= 8 && rows / s >= 1024; ++s) {
+    const double t = round_s / s * ((tiles * s + pairs - 1) / pairs) + s * piece_s;
+    if (t < best_s) {
+      best = s;
+      best_s = t;
+    }
+  }
+  return best;
+}
+
+// dw (e, n, k) = dy (e, rows, n)^T x (e, rows, k); mode: VMOE_GRAD_*.
+int weight_gradient(const void* dy, const void* x, int64_t e, int64_t rows, int64_t n, int64_t k,
+                    void* dw, int mode, float* pieces, cudaStream_t stream) {
+  const size_t width = mode == VMOE_GRAD_BF16 ? 2 : 4;
+  if (rows == 0) {
+    if (mode != VMOE_GRAD_ADD) cudaMemsetAsync(dw, 0, static_cast<size_t>(e * n * k) * width, stream);
+    return check_launch();
+  }
+  VmoeGemmArgs g;
+  const int cut = gradient_pieces(e, n, k, rows);
+  if (cut == 1) {
+    gemm_operands(&g, dy, n, rows * n, 1, x, k, rows * k, 1, n, k, rows, e);
+    g.C = dw;
+    g.c_fp32 = mode != VMOE_GRAD_BF16;
+    g.c_atomic = mode == VMOE_GRAD_ADD;
+    return vmoe_gemm_bf16(&g, stream);
+  }
+  const int64_t piece = rows / cut, left = rows % cut;
+  gemm_operands(&g, dy, n, piece * n, 1, x, k, piece * k, 1, n, k, piece, cut);
+  g.C = pieces;
+  g.c_fp32 = 1;
+  int rc = vmoe_gemm_bf16(&g, stream);
+  if (rc) return rc;
+  if (left) {
+    gemm_operands(&g, static_cast<const __nv_bfloat16*>(dy) + cut * piece * n, n, 0, 1,
+                  static_cast<const __nv_bfloat16*>(x) + cut * piece * k, k, 0, 1, n, k, left, 1);
+    g.C = pieces;
+    g.c_fp32 = 1;
+    g.c_atomic = 1;
+    if ((rc = vmoe_gemm_bf16(&g, stream))) return rc;
+  }
+  const long long count = n * k;
+  gated_join_pieces_kernel<<<static_cast<unsigned>((count / 4 + 255) / 256), 256, 0, stream>>>(
+      pieces, dw, count, cut, mode == VMOE_GRAD_BF16, mode == VMOE_GRAD_ADD);
+  return check_launch();
+}
+
+// Scratch of the backward pass, in floats: row-block sums of dg / du and of dy, gradient pieces.
+struct BackwardScratch {
+  int64_t sums, dy_sums, pieces, total;
+  explicit BackwardScratch(const VmoeGatedArgs* a) {
+    sums = a->db_in ? a->e * ((a->rows + 31) / 32) * 2 * a->m : 0;
+    dy_sums = a->db_out ? a->e * ((a->rows + ROW_BLOCK - 1) / ROW_BLOCK) * a->o : 0;
+    const int in = a->dw_in ? gradient_pieces(a->e, 2 * a->m, a->h, a->rows) : 1;
+    const int out = a->dw_out ? gradient_pieces(a->e, a->o, a->m, a->rows) : 1;
+    pieces = 0;
+    if (in > 1) pieces = in * 2 * a->m * a->h;
+    if (out > 1 && out * a->o * a->m > pieces) pieces = out * a->o * a->m;
+    sums = (sums + 3) / 4 * 4;
+    dy_sums = (dy_sums + 3) / 4 * 4;
+    total = sums + dy_sums + pieces;
+  }
+};
+
 }  // namespace
 }  // namespace vmoe
 
 using namespace vmoe;
 
+extern "C" int64_t vmoe_gated_scratch_bytes(const VmoeGatedArgs* a, int32_t backward) {
+  if (backward) return BackwardScratch(a).total * 4;
+  return a->rows > FEW_ROWS && a->b_out && a->b_out_bf16 ? a->e * a->o * 4 : 0;
+}
+
 extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  int rc = check_args(a);
+  int rc = check_sizes(a);
   if (rc) return rc;
   if (a->e == 0 || a->rows == 0) return 0;
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
+  if (a->rows <= FEW_ROWS) return few_rows(a, info, stream);
   CUtensorMap ma, mb, mh, ms;
   memset(&ms, 0, sizeof(ms));
-  if ((rc = make_bf16_map(&ma, a->a, a->k, a->rows, a->e, a->lda, a->a_batch_stride, BM, 64,
+  if ((rc = make_bf16_map(&ma, a->x, a->h, a->rows, a->e, a->h, a->rows * a->h, BM, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
-  if ((rc = make_bf16_map(&mb, a->w, a->k, a->m, 2 * a->e, a->k, a->m * a->k, HALF, 64,
+  if ((rc = make_bf16_map(&mb, a->w_in, a->h, a->m, 2 * a->e, a->h, a->m * a->h, HALF, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
   if ((rc = make_bf16_map(&mh, a->hid, a->m, a->rows, a->e, a->m, a->rows * a->m, 32, 32,
@@ -657,58 +966,98 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   if (a->saved && (rc = make_pair_map(&ms, a->saved, a->m, a->rows, a->e))) return rc;
   GatedParams p;
   memset(&p, 0, sizeof(p));
-  p.bias = a->bias;
+  p.bias = a->b_in;
+  p.bias_bf16 = a->b_in_bf16;
+  const bool convert = a->b_out && a->b_out_bf16;
+  if (convert) {
+    if (!a->scratch) return fail("gated mlp: scratch is missing");
+    p.bias_out = static_cast<const __nv_bfloat16*>(a->b_out);
+    p.bias_out_f32 = a->scratch;
+    p.bias_out_count = static_cast<int>(a->e * a->o);
+  }
   p.rows = static_cast<int>(a->rows);
-  p.k = static_cast<int>(a->k);
+  p.k = static_cast<int>(a->h);
   p.m = static_cast<int>(a->m);
   p.batch = static_cast<int>(a->e);
   p.act = a->act;
   p.save = a->saved != nullptr;
-  return launch<0>(ma, mb, mh, ms, ms, p, info, use_pairs(a, info, HALF), stream);
+  if ((rc = launch<0>(ma, mb, mh, ms, ms, p, info, use_pairs(a, info, HALF), stream))) return rc;
+  VmoeGemmArgs g;
+  gemm_operands(&g, a->hid, a->m, a->rows * a->m, 0, a->w_out, a->m, a->o * a->m, 0, a->rows, a->o, a->m,
+                a->e);
+  g.C = a->y;
+  g.bias = convert ? a->scratch : static_cast<const float*>(a->b_out);
+  g.bias_batch_stride = a->e > 1 ? a->o : 0;
+  g.residual = a->residual;
+  g.ldr = a->ld_res;
+  g.r_batch_stride = a->e > 1 ? a->res_batch_stride : 0;
+  return vmoe_gemm_bf16(&g, stream);
 }
 
-extern "C" int64_t vmoe_gated_bwd_sums_bytes(int64_t e, int64_t rows, int64_t m) {
-  return e * ((rows + 31) / 32) * 2 * m * 4;
-}
-
-extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, float* sums, float* db, int32_t accumulate,
-                              vmoe_stream_t stream_) {
+extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  int rc = check_args(a);
+  int rc = check_sizes(a);
   if (rc) return rc;
-  if (a->e == 0 || a->rows == 0) return 0;
-  if ((sums == nullptr) != (db == nullptr)) return fail("gated mlp: bias gradient needs scratch");
-  if (reinterpret_cast<uintptr_t>(sums) & 15) return fail("gated mlp: scratch must be 16-byte aligned");
+  if (a->e == 0) return 0;
+  const BackwardScratch size(a);
+  if (size.total && !a->scratch) return fail("gated mlp: scratch is missing");
+  float* sums = a->scratch;
+  float* dy_sums = a->scratch + size.sums;
+  float* pieces = dy_sums + size.dy_sums;
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
-  const bool pair = use_pairs(a, info, BN);
-  CUtensorMap ma, mb, ms, md;
-  if ((rc = make_bf16_map(&ma, a->a, a->k, a->rows, a->e, a->lda, a->a_batch_stride, BM, 64,
-                          CU_TENSOR_MAP_SWIZZLE_128B)))
-    return rc;
-  if ((rc = make_bf16_map(&mb, a->w, a->m, a->k, a->e, a->m, a->m * a->k, BK, 64,
-                          CU_TENSOR_MAP_SWIZZLE_128B)))
-    return rc;
-  if ((rc = make_pair_map(&ms, a->saved, a->m, a->rows, a->e))) return rc;
-  if ((rc = make_pair_map(&md, a->grad, a->m, a->rows, a->e))) return rc;
-  GatedParams p;
-  memset(&p, 0, sizeof(p));
-  p.sums = sums;
-  p.rows = static_cast<int>(a->rows);
-  p.k = static_cast<int>(a->k);
-  p.m = static_cast<int>(a->m);
-  p.batch = static_cast<int>(a->e);
-  if ((rc = launch<1>(ma, mb, ms, ms, md, p, info, pair, stream))) return rc;
-  if (sums) {
-    const int blocks = static_cast<int>((a->rows + 31) / 32), cols = static_cast<int>(2 * a->m);
-    if (a->e > 65535) return fail("gated mlp: too many experts");
-    gated_join_sums_kernel<<<dim3((cols + 31) / 32, static_cast<unsigned>(a->e)), 256, 0, stream>>>(
-        sums, db, blocks, cols, accumulate);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) {
-      set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
-      return -5;
-    }
+  const bool inner = a->dx || a->dw_in || a->db_in;
+  if (a->rows > 0 && a->db_out) {
+    if (a->rows > 65535ll * ROW_BLOCK) return fail("gated mlp: too many rows");
+    gated_row_sums_kernel<<<dim3(static_cast<unsigned>((a->o + 255) / 256),
+                                 static_cast<unsigned>((a->rows + ROW_BLOCK - 1) / ROW_BLOCK),
+                                 static_cast<unsigned>(a->e)),
+                            256, 0, stream>>>(static_cast<const __nv_bfloat16*>(a->dy), dy_sums,
+                                              static_cast<int>(a->rows), static_cast<int>(a->o));
+    if ((rc = check_launch())) return rc;
   }
+  if (a->rows > 0 && inner) {
+    CUtensorMap ma, mb, ms, md;
+    if ((rc = make_bf16_map(&ma, a->dy, a->o, a->rows, a->e, a->o, a->rows * a->o, BM, 64,
+                            CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
+    if ((rc = make_bf16_map(&mb, a->w_out, a->m, a->o, a->e, a->m, a->m * a->o, BK, 64,
+                            CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
+    if ((rc = make_pair_map(&ms, a->saved, a->m, a->rows, a->e))) return rc;
+    if ((rc = make_pair_map(&md, a->dgu, a->m, a->rows, a->e))) return rc;
+    GatedParams p;
+    memset(&p, 0, sizeof(p));
+    p.sums = a->db_in ? sums : nullptr;
+    p.rows = static_cast<int>(a->rows);
+    p.k = static_cast<int>(a->o);
+    p.m = static_cast<int>(a->m);
+    p.batch = static_cast<int>(a->e);
+    if ((rc = launch<1>(ma, mb, ms, ms, md, p, info, use_pairs(a, info, BN), stream))) return rc;
+  }
+  if (a->db_in || a->db_out) {
+    SumsPart u = {sums, a->db_in, static_cast<int>((a->rows + 31) / 32),
+                  a->db_in ? static_cast<int>(2 * a->m) : 0, a->db_in_mode == VMOE_GRAD_BF16,
+                  a->db_in_mode == VMOE_GRAD_ADD};
+    SumsPart v = {dy_sums, a->db_out, static_cast<int>((a->rows + ROW_BLOCK - 1) / ROW_BLOCK),
+                  a->db_out ? static_cast<int>(a->o) : 0, a->db_out_mode == VMOE_GRAD_BF16,
+                  a->db_out_mode == VMOE_GRAD_ADD};
+    gated_join_sums_kernel<<<dim3((u.cols + 31) / 32 + (v.cols + 31) / 32, static_cast<unsigned>(a->e)),
+                             256, 0, stream>>>(u, v);
+    if ((rc = check_launch())) return rc;
+  }
+  if (a->dx && a->rows > 0) {
+    VmoeGemmArgs g;
+    gemm_operands(&g, a->dgu, 2 * a->m, a->rows * 2 * a->m, 0, a->w_in, a->h, 2 * a->m * a->h, 1, a->rows,
+                  a->h, 2 * a->m, a->e);
+    g.C = a->dx;
+    if ((rc = vmoe_gemm_bf16(&g, stream))) return rc;
+  }
+  if (a->dw_in && (rc = weight_gradient(a->dgu, a->x, a->e, a->rows, 2 * a->m, a->h, a->dw_in,
+                                        a->dw_in_mode, pieces, stream)))
+    return rc;
+  if (a->dw_out && (rc = weight_gradient(a->dy, a->hid, a->e, a->rows, a->o, a->m, a->dw_out,
+                                         a->dw_out_mode, pieces, stream)))
+    return rc;
   return 0;
 }

@@ -79,29 +79,42 @@ typedef struct VmoeGemmArgs {
 VMOE_API int vmoe_gemm_bf16(const VmoeGemmArgs* args, vmoe_stream_t stream);
 
 // ----------------------------------------------------------------------------- gated MLP
-// Forward: hid (e, rows, m) = act(g) * u with g = A Wg^T + bias[0], u = A Wu^T + bias[1] per expert;
-// A (e, rows, k) bf16 with row stride lda, w (e, 2, m, k) bf16 (gate, up), bias (e, 2, m) fp32 or NULL.
-// With `saved` (e, rows, 2, m) bf16, it receives u act'(g) and act(g) for the backward pass.
-// Backward: A = dy (e, rows, k), w = w_out (e, k, m); grad (e, rows, 2, m) = (dh * saved[0],
-// dh * saved[1]) with dh = dy w, i.e. the gradients of g and u. With `sums` (scratch of
-// vmoe_gated_bwd_sums_bytes) and db (e, 2, m) fp32, db receives (accumulate: is increased by) their
-// column sums, added up in an order that does not depend on scheduling.
-// k, m, lda and a_batch_stride are multiples of 8, pointers 16-byte aligned, everything but A contiguous.
+// Per expert: y (e, rows, o) = (act(g) * u) w_out^T + b_out (+ residual) with g = x w_in[0]^T + b_in[0],
+// u = x w_in[1]^T + b_in[1]; x (e, rows, h), w_in (e, 2, m, h), w_out (e, o, m) bf16 and contiguous, biases
+// fp32 or bf16 or NULL, residual (e, rows, o) bf16 with strides or NULL. hid (e, rows, m) receives act(g) u
+// and, when set, saved (e, rows, 2, m) receives u act'(g) and act(g): both are inputs of the backward pass.
+// Backward: from dy (e, rows, o) any of dx, dw_in, dw_out (layouts of x, w_in, w_out), db_in, db_out; dgu
+// (e, rows, 2, m) is needed for the first two and db_in. All sums have a fixed order. Widths are multiples
+// of 8, pointers 16-byte aligned; scratch has vmoe_gated_scratch_bytes(args, backward) bytes, which
+// depends on the sizes and on which results are set.
+enum { VMOE_GRAD_BF16 = 0, VMOE_GRAD_F32 = 1, VMOE_GRAD_ADD = 2 };  // write bf16, fp32, add to fp32
 typedef struct VmoeGatedArgs {
-  const void* a;
-  const void* w;
-  const float* bias;
+  const void* x;
+  const void* w_in;
+  const void* b_in;
+  const void* w_out;
+  const void* b_out;
+  const void* residual;
+  void* y;
   void* hid;
   void* saved;
-  void* grad;
-  int64_t e, rows, k, m;
-  int64_t lda, a_batch_stride;
+  const void* dy;
+  void* dgu;
+  void* dx;
+  void* dw_in;
+  void* db_in;
+  void* dw_out;
+  void* db_out;
+  float* scratch;
+  int64_t e, rows, h, m, o;
+  int64_t ld_res, res_batch_stride;
   int32_t act;  // 0 GELU (tanh form), 1 SiLU
+  int32_t b_in_bf16, b_out_bf16;
+  int32_t dw_in_mode, db_in_mode, dw_out_mode, db_out_mode;  // VMOE_GRAD_*
 } VmoeGatedArgs;
+VMOE_API int64_t vmoe_gated_scratch_bytes(const VmoeGatedArgs* args, int32_t backward);
 VMOE_API int vmoe_gated_fwd(const VmoeGatedArgs* args, vmoe_stream_t stream);
-VMOE_API int64_t vmoe_gated_bwd_sums_bytes(int64_t e, int64_t rows, int64_t m);
-VMOE_API int vmoe_gated_bwd(const VmoeGatedArgs* args, float* sums, float* db, int32_t accumulate,
-                            vmoe_stream_t stream);
+VMOE_API int vmoe_gated_bwd(const VmoeGatedArgs* args, vmoe_stream_t stream);
 
 // ----------------------------------------------------------------------------- elementwise
 // LayerNorm over the last dim of bf16 x[rows][h] (h % 8 == 0, h <= 2048); gamma/beta fp32 or

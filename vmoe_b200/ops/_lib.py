@@ -7,9 +7,13 @@ implementations in ``vmoe_b200.ops`` are used and the library is optional.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
+
+import torch
+from torch import _C
 
 _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # VMOE_B200_LIB names another build of the same library (kernel experiments).
@@ -82,13 +86,12 @@ class PushArgs(ctypes.Structure):
 
 class GatedArgs(ctypes.Structure):
   """Mirror of ``VmoeGatedArgs``."""
-  _fields_ = [
-      ("a", ctypes.c_void_p), ("w", ctypes.c_void_p), ("bias", ctypes.c_void_p),
-      ("hid", ctypes.c_void_p), ("saved", ctypes.c_void_p), ("grad", ctypes.c_void_p),
-      ("e", ctypes.c_int64), ("rows", ctypes.c_int64), ("k", ctypes.c_int64),
-      ("m", ctypes.c_int64), ("lda", ctypes.c_int64), ("a_batch_stride", ctypes.c_int64),
-      ("act", ctypes.c_int32),
-  ]
+  _fields_ = [(n, ctypes.c_void_p) for n in (
+      "x", "w_in", "b_in", "w_out", "b_out", "residual", "y", "hid", "saved", "dy", "dgu", "dx",
+      "dw_in", "db_in", "dw_out", "db_out", "scratch")] + [
+          (n, ctypes.c_int64) for n in ("e", "rows", "h", "m", "o", "ld_res", "res_batch_stride")] + [
+              (n, ctypes.c_int32) for n in ("act", "b_in_bf16", "b_out_bf16", "dw_in_mode",
+                                            "db_in_mode", "dw_out_mode", "db_out_mode")]
 
 
 class DistillArgs(ctypes.Structure):
@@ -121,9 +124,20 @@ def lib() -> ctypes.CDLL:
             f"{LIB_PATH} not found: run `python -m vmoe_b200.build` (needs nvcc)")
       l = ctypes.CDLL(LIB_PATH)
       l.vmoe_last_error.restype = ctypes.c_char_p
-      l.vmoe_top_logits_max_classes.restype = ctypes.c_int64
-      l.vmoe_distill_max_classes.restype = ctypes.c_int64
-      l.vmoe_gated_bwd_sums_bytes.restype = ctypes.c_int64
+      # Entry points whose calls cost less than preparing their arguments: ctypes converts plain
+      # integers and addresses by these signatures.
+      vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+      l.vmoe_top_logits_max_classes.restype = i64
+      l.vmoe_top_logits_max_classes.argtypes = [i32]
+      l.vmoe_distill_max_classes.restype = i64
+      l.vmoe_distill_max_classes.argtypes = [i32]
+      l.vmoe_top_logits.argtypes = [vp, i32, i64, i64, i64, i64, ctypes.c_double, vp, vp, vp, vp]
+      l.vmoe_distill_fwd.argtypes = [vp, vp]
+      l.vmoe_distill_bwd.argtypes = [vp, vp, i64, vp, i64, i64, vp]
+      l.vmoe_gated_scratch_bytes.restype = i64
+      l.vmoe_gated_scratch_bytes.argtypes = [vp, i32]
+      l.vmoe_gated_fwd.argtypes = [vp, vp]
+      l.vmoe_gated_bwd.argtypes = [vp, vp]
       _lib = l
   return _lib
 
@@ -140,15 +154,15 @@ def ptr(t) -> int | None:
 
 
 def stream_ptr() -> int:
-  import torch
-  return torch.cuda.current_stream().cuda_stream
+  """The current device's current stream (the lookup that ``torch.cuda.current_stream`` wraps in a
+  Stream object, at a fiftieth of the time)."""
+  return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(t):
   """Context in which the launches for ``t`` go to its device and to that device's current
   stream (a no-op when that device is the current one already)."""
-  import contextlib
-  import torch
-  if t.device.index == torch.cuda.current_device():
-    return contextlib.nullcontext()
-  return torch.cuda.device(t.device)
+  return _HERE if t.device.index == _C._cuda_getDevice() else torch.cuda.device(t.device)

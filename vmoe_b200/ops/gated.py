@@ -1,97 +1,95 @@
-"""Gated MLP on the tcgen05 kernels (``csrc/gated_tcgen05.cu``), differentiable.
+"""Gated MLP on the GPU (``csrc/gated_tcgen05.cu``, ``csrc/gated_rows.cuh``), differentiable.
 
 ``y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wo^T + bo (+ residual)`` per expert. One kernel runs both
-projections, the activation and the product, the output projection is the library's GEMM. Backward:
-one kernel for the gradients of both projections (and their column sums), then three GEMMs for
-``dx``, ``dw_in`` and ``dw_out``. The reference has no gated MLP.
+projections, the activation and the product (a tcgen05 tile kernel, or a weight-streaming one for up
+to 16 rows); the output projection is the library's GEMM or the same streaming kernel. Backward: one
+kernel for the gradients of both projections and their column sums, then GEMMs for ``dx``, ``dw_in`` and
+``dw_out``. Each direction is one call into the library. The reference has no gated MLP.
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
 
 import torch
 import torch.nn.functional as F
 
 from vmoe_b200.ops import _lib, functional
-from vmoe_b200.ops.gemm import gemm
 
-_vp = ctypes.c_void_p
 ACTIVATIONS = {"gelu": 0, "silu": 1}
+_GRAD_BF16, _GRAD_F32, _GRAD_ADD = 0, 1, 2  # VMOE_GRAD_*
 
 
-def _args(a, w, k, m, act=0) -> "_lib.GatedArgs":
-  e, rows = a.shape[:2]
-  g = _lib.GatedArgs()
-  g.a, g.w = a.data_ptr(), w.data_ptr()
-  g.e, g.rows, g.k, g.m = e, rows, k, m
-  g.lda, g.a_batch_stride = a.stride(1), a.stride(0)
-  g.act = act
-  return g
+def _contiguous(t: torch.Tensor) -> torch.Tensor:
+  return t if t.is_contiguous() else t.contiguous()
 
 
-def _forward(x, w_in, b_in, act: int, save: bool):
-  """``(hidden (E, R, M), saved (E, R, 2, M) or None)`` of contiguous bf16 operands."""
-  e, r, h = x.shape
-  m = w_in.shape[2]
-  hid = torch.empty(e, r, m, dtype=torch.bfloat16, device=x.device)
-  saved = torch.empty(e, r, 2, m, dtype=torch.bfloat16, device=x.device) if save else None
-  g = _args(x, w_in, h, m, act)
-  g.bias, g.hid, g.saved = _lib.ptr(b_in), hid.data_ptr(), _lib.ptr(saved)
-  _lib.check(_lib.lib().vmoe_gated_fwd(ctypes.byref(g), _vp(_lib.stream_ptr())), "vmoe_gated_fwd")
-  _lib.count_launch()
-  return hid, saved
-
-
-def _backward(dy, w_out, saved, db: Optional[torch.Tensor], accumulate: bool):
-  """Gradients of both projections ``(E, R, 2, M)``; their column sums go to ``db (E, 2, M)``."""
-  e, r, o = dy.shape
-  m = saved.shape[3]
-  grad = torch.empty_like(saved)
-  g = _args(dy, w_out, o, m)
-  g.saved, g.grad = saved.data_ptr(), grad.data_ptr()
-  lib = _lib.lib()
-  sums = None
-  if db is not None:
-    size = lib.vmoe_gated_bwd_sums_bytes(ctypes.c_int64(e), ctypes.c_int64(r), ctypes.c_int64(m))
-    sums = torch.empty(size // 4, dtype=torch.float32, device=dy.device)
-  rc = lib.vmoe_gated_bwd(ctypes.byref(g), _vp(_lib.ptr(sums)), _vp(_lib.ptr(db)),
-                          ctypes.c_int32(int(accumulate)), _vp(_lib.stream_ptr()))
-  _lib.check(rc, "vmoe_gated_bwd")
-  _lib.count_launch(1 if db is None else 2)
-  return grad
-
-
-def _weight_grad(dy, x, weight, shape):
-  """``dy^T x`` for ``weight`` (viewed as ``shape``): None if added to its bound fp32 gradient, else
-  in the weight's type."""
-  e, n, k = shape
-  split = functional._wgrad_split(n, k, dy.shape[1]) if e == 1 else 1
-  tgt = functional._grad_target(weight)
-  if tgt is not None:
-    gemm(dy, x, a_mn_major=True, b_mn_major=True, out=tgt.view(shape), accumulate=True, split_k=split)
+def _bias(b):
+  if b is None:
     return None
-  if dy.shape[1] == 0:
-    return torch.zeros_like(weight)
-  if weight.dtype == torch.bfloat16 and split == 1:
-    return gemm(dy, x, a_mn_major=True, b_mn_major=True).view(weight.shape)
-  dw = torch.zeros(shape, dtype=torch.float32, device=dy.device)
-  gemm(dy, x, a_mn_major=True, b_mn_major=True, out=dw, accumulate=True, split_k=split)
-  return dw.view(weight.shape).to(weight.dtype)
+  b = b.detach()
+  return _contiguous(b if b.dtype in (torch.bfloat16, torch.float32) else b.float())
+
+
+def _weights(w: torch.Tensor) -> torch.Tensor:
+  return _contiguous(functional.bf16_shadow(w))
+
+
+def _forward(x, w_in, b_in, w_out, b_out, residual, act: int, save: bool):
+  """``(y, x, hidden, saved)`` with ``x`` as the kernels read it; the last two are inputs of the
+  backward pass (``saved`` is None without ``save``)."""
+  x = _contiguous(x)
+  w_in, w_out, b_in, b_out = _weights(w_in), _weights(w_out), _bias(b_in), _bias(b_out)
+  e, r, h = x.shape
+  _, o, m = w_out.shape
+  bf16, dev = torch.bfloat16, x.device
+  y = torch.empty((e, r, o), dtype=bf16, device=dev)
+  hid = torch.empty((e, r, m), dtype=bf16, device=dev)
+  saved = torch.empty((e, r, 2, m), dtype=bf16, device=dev) if save else None
+  g = _lib.GatedArgs()
+  g.x, g.w_in, g.w_out = x.data_ptr(), w_in.data_ptr(), w_out.data_ptr()
+  g.y, g.hid = y.data_ptr(), hid.data_ptr()
+  g.e, g.rows, g.h, g.m, g.o, g.act = e, r, h, m, o, act
+  if save:
+    g.saved = saved.data_ptr()
+  if b_in is not None:
+    g.b_in, g.b_in_bf16 = b_in.data_ptr(), b_in.dtype == bf16
+  if b_out is not None:
+    g.b_out, g.b_out_bf16 = b_out.data_ptr(), b_out.dtype == bf16
+  if residual is not None:
+    g.residual = residual.data_ptr()
+    g.res_batch_stride, g.ld_res, _ = residual.stride()
+  lib = _lib.lib()
+  if g.b_out_bf16:
+    size = lib.vmoe_gated_scratch_bytes(ctypes.byref(g), 0)
+    if size:
+      scratch = torch.empty(size // 4, dtype=torch.float32, device=dev)
+      g.scratch = scratch.data_ptr()
+  _lib.check(lib.vmoe_gated_fwd(ctypes.byref(g), _lib.stream_ptr()), "vmoe_gated_fwd")
+  _lib.count_launch(2)
+  return y, x, hid, saved
+
+
+def _gradient_of(p: torch.Tensor):
+  """``(buffer, mode, value for autograd)`` of a parameter's gradient: its bound fp32 buffer, which is
+  added to (nothing for autograd), or a new tensor in the parameter's type."""
+  tgt = functional._grad_target(p)
+  if tgt is not None:
+    return tgt, _GRAD_ADD, None
+  if p.dtype == torch.bfloat16:
+    new = torch.empty(p.shape, dtype=torch.bfloat16, device=p.device)
+    return new, _GRAD_BF16, new
+  new = torch.empty(p.shape, dtype=torch.float32, device=p.device)
+  return new, _GRAD_F32, new
 
 
 class _GatedMlpFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x, w_in, b_in, w_out, b_out, residual, act):
+    save = any(ctx.needs_input_grad[:4])
     with _lib.on_device(x):
-      x = x.contiguous()
-      w_in16, w_out16 = functional.bf16_shadow(w_in), functional.bf16_shadow(w_out)
-      b_in32 = None if b_in is None else b_in.detach().float().contiguous()
-      b_out32 = None if b_out is None else b_out.detach().float().contiguous()
-      hid, saved = _forward(x, w_in16.contiguous(), b_in32, act, any(ctx.needs_input_grad[:4]))
-      y = gemm(hid, w_out16.contiguous(), bias=b_out32, residual=residual)
-    ctx.save_for_backward(x, w_in, w_out, saved, hid if saved is not None else None)
+      y, x, hid, saved = _forward(x, w_in, b_in, w_out, b_out, residual, act, save)
+    ctx.save_for_backward(x, w_in, w_out, saved, hid if save else None)
     ctx.biases = (b_in, b_out)
     return y
 
@@ -99,33 +97,58 @@ class _GatedMlpFn(torch.autograd.Function):
   def backward(ctx, dy):
     x, w_in, w_out, saved, hid = ctx.saved_tensors
     b_in, b_out = ctx.biases
-    need = ctx.needs_input_grad
+    need_x, need_w_in, need_b_in, need_w_out, need_b_out, need_res, _ = ctx.needs_input_grad
     e, r, h = x.shape
-    m, o = w_in.shape[2], w_out.shape[1]
+    _, o, m = w_out.shape
     dx = dw_in = db_in = dw_out = db_out = None
     with _lib.on_device(x):
-      dy = dy.contiguous()
-      if need[3]:
-        dw_out = _weight_grad(dy, hid, w_out, (e, o, m))
-      if b_out is not None and need[4]:
-        db_out = functional.bias_grad(dy, b_out)
-        db_out = None if db_out is None else db_out.to(b_out.dtype)
-      if need[0] or need[1] or need[2]:
-        tgt = None
-        if b_in is not None and need[2]:
-          tgt = functional._grad_target(b_in)
-          db_in = tgt if tgt is not None else \
-              torch.zeros(e, 2, m, dtype=torch.float32, device=dy.device)
-        dgu = _backward(dy, functional.bf16_shadow(w_out).contiguous(), saved, db_in,
-                        tgt is not None).view(e, r, 2 * m)
-        if db_in is not None:
-          db_in = None if tgt is not None else db_in.to(b_in.dtype)
-        if need[0]:
-          w_in16 = functional.bf16_shadow(w_in).contiguous()
-          dx = gemm(dgu, w_in16.view(e, 2 * m, h), b_mn_major=True)
-        if need[1]:
-          dw_in = _weight_grad(dgu, x, w_in, (e, 2 * m, h))
-    return dx, dw_in, db_in, dw_out, db_out, dy if need[5] else None, None
+      dy = _contiguous(dy)
+      if dy.data_ptr() % 16:
+        dy = dy.clone()
+      dev = dy.device
+      g = _lib.GatedArgs()
+      g.x, g.dy = x.data_ptr(), dy.data_ptr()
+      g.e, g.rows, g.h, g.m, g.o = e, r, h, m, o
+      keep = []  # buffers that must live until the launches are enqueued
+      if need_x or need_w_in or need_b_in:
+        w16 = _weights(w_out)
+        dgu = torch.empty((e, r, 2, m), dtype=torch.bfloat16, device=dev)
+        g.saved, g.w_out, g.dgu = saved.data_ptr(), w16.data_ptr(), dgu.data_ptr()
+        keep += [w16, dgu]
+        launches = 1
+      else:
+        launches = 0
+      if need_x:
+        w16 = _weights(w_in)
+        dx = torch.empty((e, r, h), dtype=torch.bfloat16, device=dev)
+        g.w_in, g.dx = w16.data_ptr(), dx.data_ptr()
+        keep.append(w16)
+      if need_w_in:
+        buf, g.dw_in_mode, dw_in = _gradient_of(w_in)
+        g.dw_in = buf.data_ptr()
+        keep.append(buf)
+      if need_w_out:
+        buf, g.dw_out_mode, dw_out = _gradient_of(w_out)
+        g.dw_out, g.hid = buf.data_ptr(), hid.data_ptr()
+        keep.append(buf)
+      if need_b_in:
+        buf, g.db_in_mode, db_in = _gradient_of(b_in)
+        g.db_in = buf.data_ptr()
+        keep.append(buf)
+      if need_b_out:
+        buf, g.db_out_mode, db_out = _gradient_of(b_out)
+        g.db_out = buf.data_ptr()
+        keep.append(buf)
+      lib = _lib.lib()
+      size = lib.vmoe_gated_scratch_bytes(ctypes.byref(g), 1)
+      if size:
+        keep.append(torch.empty(size // 4, dtype=torch.float32, device=dev))
+        g.scratch = keep[-1].data_ptr()
+      if launches or need_w_out or need_b_out:
+        _lib.check(lib.vmoe_gated_bwd(ctypes.byref(g), _lib.stream_ptr()), "vmoe_gated_bwd")
+        _lib.count_launch(launches + int(need_x) + int(need_w_in) + int(need_w_out) +
+                          int(need_b_out) + int(need_b_in or need_b_out))
+    return dx, dw_in, db_in, dw_out, db_out, dy if need_res else None, None
 
 
 def gated_reference(x, w_in, b_in, w_out, b_out, act: str, residual=None):
@@ -151,20 +174,21 @@ def check_args(x, w_in, b_in, w_out, b_out, act, residual) -> None:
                      f"{tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
   e, r, h = x.shape
   m, o = w_in.shape[2], w_out.shape[1]
-  if tuple(w_in.shape) != (e, 2, m, h) or tuple(w_out.shape) != (e, o, m) or min(h, m, o) < 1:
+  if w_in.shape != (e, 2, m, h) or w_out.shape != (e, o, m) or min(h, m, o) < 1:
     raise ValueError("expert_gated_mlp: x (E, R, H), w_in (E, 2, M, H) and w_out (E, O, M) do not fit "
                      f"together: {tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
-  for name, t, shape in (("b_in", b_in, (e, 2, m)), ("b_out", b_out, (e, o)),
-                         ("residual", residual, (e, r, o))):
-    if t is not None and tuple(t.shape) != shape:
-      raise ValueError(f"expert_gated_mlp: {name} must be {shape}, got {tuple(t.shape)}")
   if residual is not None and residual.dtype != x.dtype:
     raise TypeError(f"expert_gated_mlp: residual must be {x.dtype} like x, got {residual.dtype}")
-  for name, t in (("w_in", w_in), ("b_in", b_in), ("w_out", w_out), ("b_out", b_out),
-                  ("residual", residual)):
-    if t is not None and t.device != x.device:
-      raise ValueError(f"expert_gated_mlp: {name} is on {t.device}, x on {x.device}")
-    if t is not None and not t.dtype.is_floating_point:
+  dev = x.device
+  for name, t, shape in (("w_in", w_in, None), ("b_in", b_in, (e, 2, m)), ("w_out", w_out, None),
+                         ("b_out", b_out, (e, o)), ("residual", residual, (e, r, o))):
+    if t is None:
+      continue
+    if shape is not None and t.shape != shape:
+      raise ValueError(f"expert_gated_mlp: {name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != dev:
+      raise ValueError(f"expert_gated_mlp: {name} is on {t.device}, x on {dev}")
+    if not t.is_floating_point():
       raise TypeError(f"expert_gated_mlp: {name} must be floating point, got {t.dtype}")
 
 
@@ -180,7 +204,15 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, act: str, residual=None) -> torch.Ten
     b_in = None if b_in is None else F.pad(b_in, (0, mp))
     b_out = None if b_out is None else F.pad(b_out, (0, op))
     residual = None if residual is None else F.pad(residual, (0, op))
-  if residual is not None and (residual.stride(-1) != 1 or residual.stride(-2) % 8):
+  if residual is not None and (residual.stride(2) != 1 or residual.stride(1) % 8 or
+                               residual.stride(0) % 8 or residual.data_ptr() % 16):
     residual = residual.contiguous()
-  y = _GatedMlpFn.apply(x, w_in, b_in, w_out, b_out, residual, ACTIVATIONS[act])
+  if x.data_ptr() % 16:  # a view that starts inside 16 bytes
+    x = x.clone()
+  args = (x, w_in, b_in, w_out, b_out, residual)
+  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    y = _GatedMlpFn.apply(*args, ACTIVATIONS[act])
+  else:
+    with _lib.on_device(x):
+      y = _forward(*args, ACTIVATIONS[act], False)[0]
   return y[..., :o] if op else y

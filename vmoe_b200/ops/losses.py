@@ -88,29 +88,39 @@ class TopLogits(NamedTuple):
   rest: torch.Tensor     # (rows,) fp32
 
 
-def _check_logits(logits, what: str) -> None:
+def _check_logits(logits, temperature, what: str) -> float:
   if logits.dim() != 2:
     raise ValueError(f"{what}: logits must be (rows, classes), got shape {tuple(logits.shape)}")
-  if not logits.dtype.is_floating_point:
+  if not logits.is_floating_point():
     raise TypeError(f"{what}: logits must be floating point, got {logits.dtype}")
   if logits.shape[1] < 1:
     raise ValueError(f"{what}: there must be at least one class")
-
-
-def _check_temperature(temperature, what: str) -> float:
   temperature = float(temperature)
   if not 1e-3 <= temperature <= 1e3:
     raise ValueError(f"{what}: temperature must be in [1e-3, 1e3], got {temperature}")
   return temperature
 
 
-def _on_kernels(logits) -> bool:
-  return (functional.cuda_kernels_enabled() and logits.is_cuda and logits.dtype in _FLOAT_CODES)
+_MAX_CLASSES: dict = {}
+
+
+def _on_kernels(logits, what: str) -> bool:
+  """Whether the kernels take these logits (type, device, classes that fit shared memory)."""
+  if not (functional.cuda_kernels_enabled() and logits.is_cuda):
+    return False
+  code = _FLOAT_CODES.get(logits.dtype)
+  if code is None:
+    return False
+  most = _MAX_CLASSES.get((what, code))
+  if most is None:
+    most = getattr(_lib.lib(), f"vmoe_{what}_max_classes")(code)
+    _MAX_CLASSES[what, code] = most
+  return logits.shape[1] <= most
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
   """``t`` with contiguous rows (any distance between them)."""
-  return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+  return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -124,29 +134,24 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0) -> Top
   +inf. ``rest`` is ``logsumexp(logits / temperature)`` over the classes that are not among them,
   ``-inf`` when there are none. No gradient: this is the frozen side of ``distill_xent``.
   """
-  _check_logits(logits, "top_logits")
-  temperature = _check_temperature(temperature, "top_logits")
+  temperature = _check_logits(logits, temperature, "top_logits")
   rows, n = logits.shape
   if not 1 <= k <= min(n, TOP_LOGITS_MAX):
     raise ValueError(f"top_logits: k must be in 1 .. {min(n, TOP_LOGITS_MAX)}, got {k}")
+  if _on_kernels(logits, "top_logits"):
+    with _lib.on_device(logits):
+      x = _rows(logits)
+      dev = x.device
+      values = torch.empty((rows, k), dtype=x.dtype, device=dev)
+      indices = torch.empty((rows, k), dtype=torch.int32, device=dev)
+      rest = torch.empty(rows, dtype=torch.float32, device=dev)
+      rc = _lib.lib().vmoe_top_logits(
+          x.data_ptr(), _FLOAT_CODES[x.dtype], rows, n, _ld(x), k, temperature, values.data_ptr(),
+          indices.data_ptr(), rest.data_ptr(), _lib.stream_ptr())
+      _lib.check(rc, "vmoe_top_logits")
+      _lib.count_launch()
+    return TopLogits(values, indices, rest)
   logits = logits.detach()
-  if _on_kernels(logits):
-    lib = _lib.lib()
-    code = _FLOAT_CODES[logits.dtype]
-    if n <= lib.vmoe_top_logits_max_classes(ctypes.c_int32(code)):
-      with _lib.on_device(logits):
-        x = _rows(logits)
-        values = torch.empty(rows, k, dtype=x.dtype, device=x.device)
-        indices = torch.empty(rows, k, dtype=torch.int32, device=x.device)
-        rest = torch.empty(rows, dtype=torch.float32, device=x.device)
-        rc = lib.vmoe_top_logits(
-            _vp(x.data_ptr()), ctypes.c_int32(code), ctypes.c_int64(rows), ctypes.c_int64(n),
-            ctypes.c_int64(_ld(x)), ctypes.c_int64(k), ctypes.c_double(temperature),
-            _vp(values.data_ptr()), _vp(indices.data_ptr()), _vp(rest.data_ptr()),
-            _vp(_lib.stream_ptr()))
-        _lib.check(rc, "vmoe_top_logits")
-        _lib.count_launch()
-      return TopLogits(values, indices, rest)
   x = logits.float()
   order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :k]
   others = (x / temperature).scatter(1, order, -math.inf)
@@ -160,48 +165,50 @@ class _DistillFn(torch.autograd.Function):
     with _lib.on_device(logits):
       rows, n = logits.shape
       x = _rows(logits)
+      k = values.shape[1]
       dev = x.device
       a = _lib.DistillArgs()
       loss = torch.empty(rows, dtype=torch.float32, device=dev)
-      stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
-      slopes = torch.empty(rows, values.shape[1], dtype=torch.float32, device=dev)
+      kept = torch.empty((k + 2) * rows, dtype=torch.float32, device=dev)  # stats, slopes
       a.logits, a.values, a.indices = x.data_ptr(), values.data_ptr(), indices.data_ptr()
-      a.rest = _lib.ptr(rest)
-      a.loss, a.stats, a.slopes = loss.data_ptr(), stats.data_ptr(), slopes.data_ptr()
-      a.rows, a.n, a.k = rows, n, values.shape[1]
+      if rest is not None:
+        a.rest = rest.data_ptr()
+      a.loss, a.stats = loss.data_ptr(), kept.data_ptr()
+      a.slopes = kept.data_ptr() + 8 * rows
+      a.rows, a.n, a.k, a.temperature = rows, n, k, temperature
       a.ld, a.ld_values, a.ld_indices = _ld(x), _ld(values), _ld(indices)
-      a.temperature = temperature
       a.dtype, a.values_dtype = _FLOAT_CODES[x.dtype], _FLOAT_CODES[values.dtype]
-      a.indices_wide = int(indices.dtype == torch.int64)
-      rc = _lib.lib().vmoe_distill_fwd(ctypes.byref(a), _vp(_lib.stream_ptr()))
-      _lib.check(rc, "vmoe_distill_fwd")
+      a.indices_wide = indices.dtype == torch.int64
+      _lib.check(_lib.lib().vmoe_distill_fwd(ctypes.byref(a), _lib.stream_ptr()),
+                 "vmoe_distill_fwd")
       _lib.count_launch()
-    ctx.save_for_backward(x, indices, stats, slopes)
+    ctx.save_for_backward(x, indices, kept)
     ctx.args = a
     return loss
 
   @staticmethod
   def backward(ctx, dloss):
-    x, indices, stats, slopes = ctx.saved_tensors
+    x, _, _ = ctx.saved_tensors
     a = ctx.args
-    rows, n = x.shape
+    rows, n, dtype = a.rows, a.n, x.dtype
     with _lib.on_device(x):
       # Gradient rows keep the logits' place within 16 bytes, so that both sides move in the same
       # vectors; the padding of padded rows (a classification head whose width is not a multiple
       # of 8) is zeroed.
-      size = x.element_size()
-      width = 16 // size
-      phase = x.data_ptr() % 16 // size
-      ld = n + (a.ld - n) % width
-      buf = torch.empty(phase + rows * ld, dtype=x.dtype, device=x.device)
-      grad = buf[phase:].view(rows, ld)
-      d = dloss if dloss.dtype == torch.float32 else dloss.float()
-      rc = _lib.lib().vmoe_distill_bwd(
-          ctypes.byref(a), _vp(d.data_ptr()), ctypes.c_int64(d.stride(0)), _vp(grad.data_ptr()),
-          ctypes.c_int64(ld), ctypes.c_int64(ld), _vp(_lib.stream_ptr()))
+      size = 4 if dtype == torch.float32 else 2
+      ld = n + (a.ld - n) % (16 // size)
+      phase = a.logits % 16 // size if rows else 0
+      if phase:
+        grad = torch.empty(phase + rows * ld, dtype=dtype, device=x.device)[phase:].view(rows, ld)
+      else:
+        grad = torch.empty((rows, ld), dtype=dtype, device=x.device)
+      if dloss.dtype != torch.float32:
+        dloss = dloss.float()
+      rc = _lib.lib().vmoe_distill_bwd(ctypes.byref(a), dloss.data_ptr(), dloss.stride(0),
+                                       grad.data_ptr(), ld, ld, _lib.stream_ptr())
       _lib.check(rc, "vmoe_distill_bwd")
       _lib.count_launch()
-    return grad[:, :n], None, None, None, None
+    return grad if ld == n else grad[:, :n], None, None, None, None
 
 
 def _distill_reference(logits, values, indices, rest, temperature):
@@ -245,8 +252,7 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
   An example whose incoming gradient is 0 gets a zero gradient whatever its logits hold. Gradients
   flow to ``logits`` only.
   """
-  _check_logits(logits, "distill_xent")
-  temperature = _check_temperature(temperature, "distill_xent")
+  temperature = _check_logits(logits, temperature, "distill_xent")
   rows, n = logits.shape
   if values.dim() != 2 or values.shape[0] != rows or values.shape[1] < 1:
     raise ValueError(f"distill_xent: values must be ({rows}, k >= 1), got {tuple(values.shape)}")
@@ -255,19 +261,18 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
                      f"{tuple(indices.shape)} and {tuple(values.shape)}")
   if indices.dtype not in (torch.int32, torch.int64):
     raise TypeError(f"distill_xent: indices must be int32 or int64, got {indices.dtype}")
-  if not values.dtype.is_floating_point:
+  if not values.is_floating_point():
     raise TypeError(f"distill_xent: values must be floating point, got {values.dtype}")
-  if rest is not None and tuple(rest.shape) != (rows,):
+  if rest is not None and rest.shape != (rows,):
     raise ValueError(f"distill_xent: rest must be ({rows},), got {tuple(rest.shape)}")
-  for name, t in (("values", values), ("indices", indices), ("rest", rest)):
-    if t is not None and t.device != logits.device:
-      raise ValueError(f"distill_xent: {name} is on {t.device}, logits on {logits.device}")
-  values, rest = values.detach(), None if rest is None else rest.detach()
-  if (_on_kernels(logits) and values.shape[1] <= 65535 and
-      n <= _lib.lib().vmoe_distill_max_classes(ctypes.c_int32(_FLOAT_CODES[logits.dtype]))):
+  dev = logits.device
+  if values.device != dev or indices.device != dev or (rest is not None and rest.device != dev):
+    raise ValueError(f"distill_xent: values, indices and rest must be on {dev} like logits")
+  if _on_kernels(logits, "distill") and values.shape[1] <= 65535:
     if values.dtype not in _FLOAT_CODES:
       values = values.float()
-    if rest is not None:
+    if rest is not None and (rest.dtype != torch.float32 or not rest.is_contiguous()):
       rest = rest.to(torch.float32).contiguous()
     return _DistillFn.apply(logits, _rows(values), _rows(indices), rest, temperature)
+  values, rest = values.detach(), None if rest is None else rest.detach()
   return _distill_reference(logits, values, indices, rest, temperature)
