@@ -237,6 +237,21 @@ struct Max {
   __device__ __forceinline__ double operator()(double a, double b) const { return a > b || a != a ? a : b; }
 };
 
+// Adds the warp's counts to a counter in shared memory with one atomic (they queue up on one address:
+// 250 of them cost 10 000 cycles) and returns where this lane's share starts.
+__device__ __forceinline__ int claim(int* counter, int mine) {
+  const int lane = threadIdx.x & 31;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  int base = 0;
+  if (lane == 31 && upto) base = atomicAdd(counter, upto);
+  return __shfl_sync(0xffffffffu, base, 31) + upto - mine;
+}
+
 // The vectors v0 .. v1 - 1 of a row that belong to this CTA, on their way to shared memory. Vector j
 // holds the elements j W - off .. j W - off + W - 1 (off: the row's place within 16 bytes).
 template <typename T, int DT>
@@ -403,19 +418,24 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     const float anchor = near ? -m * c : 0.0f;
     f32x2 acc = 0;
     u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-50
-    auto take_apart = [&](int j, const uint4& q) {
+    // Candidates of the vector j (none if `has` is false); all lanes of a warp take part.
+    auto take_apart = [&](bool has, int j, const uint4& q) {
+      uint32_t hits = 0;
+      if (has) {
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const uint32_t key = Ord::key(bits_at<T>(q, e));
-        const int at = st.position(j, e);
-        if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
-        if (taken(key, at)) {
-          const int pos = atomicAdd(&count, 1);
-          if (pos < TOP_CAP)
-            cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
-        } else if (near) {
-          odd += __float2ull_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p50f);
+        for (int e = 0; e < W; ++e) {
+          const uint32_t key = Ord::key(bits_at<T>(q, e));
+          const int at = st.position(j, e);
+          if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
+          if (taken(key, at)) hits |= 1u << e;
+          else if (near) odd += __float2ull_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p50f);
         }
+      }
+      int pos = claim(&count, __popc(hits));
+      for (; hits && pos < TOP_CAP; hits &= hits - 1, ++pos) {
+        const int e = __ffs(hits) - 1;
+        cand[pos] = (static_cast<u64>(Ord::key(bits_at<T>(q, e))) << 32) |
+                    (0xffffffffu - static_cast<uint32_t>(st.position(j, e)));
       }
     };
     if (attempt == 0) {
@@ -428,22 +448,31 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
         if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) acc = f2_add(acc, sum);
         else mine_hot |= 1ull << i;
       }
-      if (mine_hot) {
-        int pos = atomicAdd(&hot_count, __popcll(mine_hot));
-        for (; mine_hot && pos < TOP_CAP; mine_hot &= mine_hot - 1, ++pos)
-          hot[pos] = tid + (__ffsll(mine_hot) - 1) * DT;
-      }
+      int pos = claim(&hot_count, __popcll(mine_hot));
+      for (; mine_hot && pos < TOP_CAP; mine_hot &= mine_hot - 1, ++pos)
+        hot[pos] = tid + (__ffsll(mine_hot) - 1) * DT;
     } else {  // exact bounds: any number of vectors may hold values equal to the bound
-      for (int j = tid; j < nv; j += DT) {
-        const uint4 q = st.row[j];
-        if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) acc = f2_add(acc, exponentials<T>(q, c, anchor));
-        else take_apart(j, q);
+      for (int j0 = 0; j0 < nv; j0 += DT) {
+        const int j = j0 + tid;
+        const uint4 q = j < nv ? st.row[j] : make_uint4(0, 0, 0, 0);
+        const bool below = j < nv && Ord::all_below(Ord::largest(Ord::kLow, q), m);
+        if (below) acc = f2_add(acc, exponentials<T>(q, c, anchor));
+        take_apart(j < nv && !below, j, q);
       }
     }
     __syncthreads();
-    if (hot_count <= TOP_CAP)
-      for (int h = tid; h < hot_count; h += DT) take_apart(hot[h], st.row[hot[h]]);
-    if (odd) atomicAdd(&odd_sum, odd);  // integers: the order does not matter
+    if (hot_count <= TOP_CAP) {
+      for (int h0 = 0; h0 < hot_count; h0 += DT) {
+        const int h = h0 + tid;
+        const bool has = h < hot_count;
+        if (!__any_sync(0xffffffffu, has)) break;  // whole warps only
+        const int j = has ? hot[h] : 0;
+        take_apart(has, j, st.row[j]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    if (odd && (tid & 31) == 0) atomicAdd(&odd_sum, odd);  // integers: the order does not matter
     float s0, s1;
     f2_unpack(acc, s0, s1);
     s = near ? s0 + s1 : 0.0f;
@@ -589,28 +618,29 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   for (int q = mine + tid; q < k; q += DT) sorted[q] = 0;
   cluster_sync_all();
   u64* lists = reinterpret_cast<u64*>(row_smem) + list_offset;  // [parts][k] behind the row
-  for (int q = tid; q < parts * k; q += DT) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];"
-                 : "=l"(v)
-                 : "r"(mapa_shared(smem_u32(sorted + q % k), static_cast<uint32_t>(q / k))));
-    lists[q] = v;
+  for (int p = tid >> 5; p < parts; p += DT / 32) {
+    const uint32_t src = mapa_shared(smem_u32(sorted), static_cast<uint32_t>(p));
+    for (int q = tid & 31; q < k; q += 32) {
+      u64 v;
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(src + 8u * q));
+      lists[p * k + q] = v;
+    }
   }
   __syncthreads();
   uint32_t out_key = 0;
   if (tid < mine) {  // k <= 256 <= DT
     const u64 me = sorted[tid];
-    int rank = tid;
-    for (int p = 0; p < parts; ++p) {
-      if (p == part) continue;
-      int lo = 0, hi = k;  // first position whose entry is smaller
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (lists[p * k + mid] > me) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
+    // In every list the first position whose entry is not larger, all lists in step.
+    int at[MAX_PARTS] = {};
+#pragma unroll 1
+    for (int step = 256; step > 0; step >>= 1) {
+#pragma unroll
+      for (int p = 0; p < MAX_PARTS; ++p)
+        if (p < parts && at[p] + step <= k && lists[p * k + at[p] + step - 1] > me) at[p] += step;
     }
+    int rank = 0;  // this CTA's own list counts its place
+#pragma unroll
+    for (int p = 0; p < MAX_PARTS; ++p) rank += at[p];
     if (rank < k) emit(rank, me);
     else out_key = static_cast<uint32_t>(me >> 32);
   }
