@@ -299,6 +299,10 @@ struct StagedRow {
   __device__ __forceinline__ bool holds(int position) const {
     return position >= 0 && position < n && position + off >= v0 * W && position + off < v1 * W;
   }
+  __device__ __forceinline__ uint32_t bits(int position) const {
+    using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, unsigned short>::type;
+    return reinterpret_cast<const Bits*>(row)[position + off - v0 * W];
+  }
   __device__ __forceinline__ T at(int position) const {
     return reinterpret_cast<const T*>(row)[position + off - v0 * W];
   }
@@ -307,7 +311,7 @@ struct StagedRow {
 // ------------------------------------------------------------------------------- top logits
 constexpr int TOP_K_MAX = 256;
 
-// The k largest of the threads' maxima (found by one warp's bisection on their order keys) bound the
+// The k largest of the threads' maxima (found by bisection on their order keys) bound the
 // k-th largest value from below, so everything not below that bound is a candidate: somewhat more
 // than k of them for values in no particular order. Where there are too many (more kept than
 // threads, rows of equal values) the bisection goes on over all values, and over positions among
@@ -333,7 +337,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   __shared__ float2 part_rest[MAX_PARTS];
   __shared__ __align__(8) uint64_t bar_mem;
   __shared__ int count, hot_count, gave_up;
-  __shared__ uint32_t first_bound;
+  __shared__ uint2 red_range[DT / 32];
+  __shared__ u64 part_bound[MAX_PARTS];
+  __shared__ int list_length[MAX_PARTS];
   __shared__ u64 odd_sum;
   const int tid = threadIdx.x;
   const int part = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -354,57 +360,32 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     m1 = Ord::largest(m1, st.row[i + DT]);
   }
   if (i < nv) m0 = Ord::largest(m0, st.row[i]);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(cand);
-  keys[tid] = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
-  __syncthreads();
+  const uint32_t best = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
 
   // Bound: at least `mine` elements have a key >= bound (0: all elements).
-  if (tid < 32) {
-    uint32_t own[DT / 32], lo = 0xffffffffu, hi = 0;
-    int filled = 0;
+  uint32_t bound = 0;
+  if (__syncthreads_count(best != 0) >= mine && mine > 0) {
+    uint32_t lo = __reduce_min_sync(0xffffffffu, best ? best : 0xffffffffu);
+    uint32_t hi = __reduce_max_sync(0xffffffffu, best);
+    if ((tid & 31) == 0) red_range[tid >> 5] = make_uint2(lo, hi);
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < DT / 32; ++q) {
-      own[q] = keys[tid + 32 * q];
-      hi = max(hi, own[q]);
-      if (own[q]) lo = min(lo, own[q]), ++filled;
+      lo = min(lo, red_range[q].x);
+      hi = max(hi, red_range[q].y);
     }
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    filled = __reduce_add_sync(0xffffffffu, filled);
-    if (filled < mine || mine == 0) lo = hi = 0;
-    // count(>= lo) >= mine, the bound is <= hi. Three counts per step, in one word: a quarter of the
-    // range is left for the time of one reduction.
-    while (lo < hi) {
-      const uint32_t step = (hi - lo) / 4;
-      const uint32_t m1 = lo + step + 1, m2 = m1 + step, m3 = min(m2 + step, hi);
-      uint32_t got = 0;
-#pragma unroll
-      for (int q = 0; q < DT / 32; ++q)
-        got += (own[q] >= m1 ? 1u : 0u) + (own[q] >= m2 ? 1u << 10 : 0u) + (own[q] >= m3 ? 1u << 20 : 0u);
-      got = __reduce_add_sync(0xffffffffu, got);
-      const int g1 = got & 1023, g2 = (got >> 10) & 1023, g3 = got >> 20;
-      int g;
-      if (g3 >= mine) {
-        lo = m3;
-        g = g3;
-      } else if (g2 >= mine) {
-        lo = m2;
-        hi = m3 - 1;
-        g = g2;
-      } else if (g1 >= mine) {
-        lo = m1;
-        hi = m2 - 1;
-        g = g1;
+    while (lo < hi) {  // count(>= lo) >= mine; the bound is <= hi
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      const int got = __syncthreads_count(best >= mid);
+      if (got >= mine) {
+        lo = mid;
+        if (got <= mine + mine / 8 + 4) break;
       } else {
-        hi = m1 - 1;
-        continue;
+        hi = mid - 1;
       }
-      if (g <= mine + mine / 8 + 4) break;
     }
-    if (tid == 0) first_bound = lo;
+    bound = lo;
   }
-  __syncthreads();
-  uint32_t bound = first_bound;
 
   int last_at = 0x7fffffff;  // elements equal to the bound count up to this position
   auto taken = [&](uint32_t key, int at) { return key > bound || (key == bound && at <= last_at); };
@@ -417,25 +398,25 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     const bool near = fabsf(m) < FAR;
     const float anchor = near ? -m * c : 0.0f;
     f32x2 acc = 0;
-    u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-50
+    u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-31
     // Candidates of the vector j (none if `has` is false); all lanes of a warp take part.
-    auto take_apart = [&](bool has, int j, const uint4& q) {
+    auto take_apart = [&](bool has, int j) {
       uint32_t hits = 0;
       if (has) {
+        const uint4 q = st.row[j];
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           const uint32_t key = Ord::key(bits_at<T>(q, e));
           const int at = st.position(j, e);
           if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
           if (taken(key, at)) hits |= 1u << e;
-          else if (near) odd += __float2ull_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p50f);
+          else if (near) odd += __float2uint_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p31f);
         }
       }
       int pos = claim(&count, __popc(hits));
       for (; hits && pos < TOP_CAP; hits &= hits - 1, ++pos) {
-        const int e = __ffs(hits) - 1;
-        cand[pos] = (static_cast<u64>(Ord::key(bits_at<T>(q, e))) << 32) |
-                    (0xffffffffu - static_cast<uint32_t>(st.position(j, e)));
+        const int at = st.position(j, __ffs(hits) - 1);
+        cand[pos] = (static_cast<u64>(Ord::key(st.bits(at))) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
       }
     };
     if (attempt == 0) {
@@ -457,7 +438,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
         const uint4 q = j < nv ? st.row[j] : make_uint4(0, 0, 0, 0);
         const bool below = j < nv && Ord::all_below(Ord::largest(Ord::kLow, q), m);
         if (below) acc = f2_add(acc, exponentials<T>(q, c, anchor));
-        take_apart(j < nv && !below, j, q);
+        take_apart(j < nv && !below, j);
       }
     }
     __syncthreads();
@@ -466,8 +447,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
         const int h = h0 + tid;
         const bool has = h < hot_count;
         if (!__any_sync(0xffffffffu, has)) break;  // whole warps only
-        const int j = has ? hot[h] : 0;
-        take_apart(has, j, st.row[j]);
+        take_apart(has, has ? hot[h] : 0);
       }
     }
 #pragma unroll
@@ -540,7 +520,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   }
   s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
   if (fabsf(m) < FAR)  // the last factor takes the rounding of m c back
-    s = (s + static_cast<float>(odd_sum) * 0x1p-50f) * exp2_approx(-fmaf(m, c, -m * c));
+    s = (s + static_cast<float>(odd_sum) * 0x1p-31f) * exp2_approx(-fmaf(m, c, -m * c));
   // Adds values (each thread's own, through `each`) whose largest key is `key` to the sum; none of
   // them lies below what is in the sum already.
   auto add_at = [&](uint32_t key, auto each) {
@@ -574,9 +554,9 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
       s = (s > 0.0f ? s * exp2_approx((m - top_value) * c) : s) + t;
       m = top_value;
     }
-  } else if (s < 1e-8f) {
-    // Nothing, or all of it far below the bound (where the units of odd_sum and, further down, fp32
-    // itself would show): anchor at the largest of it.
+  } else if (s < 0.125f) {
+    // Nothing, or all of it below the bound by so much that the units of odd_sum and, further down,
+    // fp32 itself would show: anchor at the largest of it.
     auto walk = [&](auto visit) {
       for (int j = tid; j < nv; j += DT) {
         const uint4 q = st.row[j];
@@ -612,35 +592,57 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     return;
   }
 
-  // The parts' sorted lists meet: an entry's place in the row is its place here plus the number
-  // of larger entries in the other lists.
-  __syncthreads();
+  // The parts' sorted lists meet. Every part has ceil(k / parts) entries that are not below the least of
+  // the parts' entries at that place, so nothing below it can be among the k largest of the row: little
+  // more than k entries are left. An entry's place in the row is its place here plus the number of
+  // larger entries in the other lists.
+  const int place = (k + parts - 1) / parts - 1;
+  if (tid < parts) {
+    const u64 v = place < mine ? sorted[place] : 0;
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(
+                     mapa_shared(smem_u32(part_bound + part), static_cast<uint32_t>(tid))),
+                 "l"(v)
+                 : "memory");
+  }
   for (int q = mine + tid; q < k; q += DT) sorted[q] = 0;
   cluster_sync_all();
+  u64 floor_entry = part_bound[0];
+  for (int p = 1; p < parts; ++p) floor_entry = min(floor_entry, part_bound[p]);
   u64* lists = reinterpret_cast<u64*>(row_smem) + list_offset;  // [parts][k] behind the row
   for (int p = tid >> 5; p < parts; p += DT / 32) {
     const uint32_t src = mapa_shared(smem_u32(sorted), static_cast<uint32_t>(p));
-    for (int q = tid & 31; q < k; q += 32) {
-      u64 v;
-      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(src + 8u * q));
-      lists[p * k + q] = v;
+    int length = 0;
+    for (int q0 = 0; q0 < k; q0 += 32) {
+      const int q = q0 + (tid & 31);
+      u64 v = 0;
+      if (q < k) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(src + 8u * q));
+      const bool in = v != 0 && v >= floor_entry;
+      if (in) lists[p * k + q] = v;
+      const uint32_t mask = __ballot_sync(0xffffffffu, in);
+      length += __popc(mask);
+      if (mask != 0xffffffffu) break;
     }
+    if ((tid & 31) == 0) list_length[p] = length;
   }
   __syncthreads();
   uint32_t out_key = 0;
   if (tid < mine) {  // k <= 256 <= DT
     const u64 me = sorted[tid];
-    // In every list the first position whose entry is not larger, all lists in step.
-    int at[MAX_PARTS] = {};
+    int rank = k;
+    if (me >= floor_entry) {
+      // In every list the first position whose entry is not larger, all lists in step.
+      int at[MAX_PARTS] = {};
 #pragma unroll 1
-    for (int step = 256; step > 0; step >>= 1) {
+      for (int step = 256; step > 0; step >>= 1) {
 #pragma unroll
-      for (int p = 0; p < MAX_PARTS; ++p)
-        if (p < parts && at[p] + step <= k && lists[p * k + at[p] + step - 1] > me) at[p] += step;
+        for (int p = 0; p < MAX_PARTS; ++p)
+          if (p < parts && at[p] + step <= list_length[p] && lists[p * k + at[p] + step - 1] > me)
+            at[p] += step;
+      }
+      rank = 0;  // this CTA's own list counts its place
+#pragma unroll
+      for (int p = 0; p < MAX_PARTS; ++p) rank += at[p];
     }
-    int rank = 0;  // this CTA's own list counts its place
-#pragma unroll
-    for (int p = 0; p < MAX_PARTS; ++p) rank += at[p];
     if (rank < k) emit(rank, me);
     else out_key = static_cast<uint32_t>(me >> 32);
   }
@@ -678,8 +680,10 @@ __device__ __forceinline__ int load_index(const void* p, int wide, long long i, 
   return v >= 0 && v < n ? static_cast<int>(v) : -1;
 }
 
-constexpr int FT = 256;       // threads of the forward and backward kernels
-constexpr int ENTRIES = 128;  // kept classes whose logits stay in shared memory
+constexpr int ST = 128;            // threads of the forward kernels
+constexpr int FT = 256;            // threads of the backward kernel
+constexpr int ENTRIES = 64;        // kept classes whose logits stay in shared memory
+constexpr int MAX_SUM_PARTS = 32;  // parts of a row in the sums kernel
 
 struct DistillParams {
   const void* values;
@@ -689,6 +693,8 @@ struct DistillParams {
   float2* stats;      // per row: anchor and factor of the classes that are not kept
   float* slopes;      // per kept class: student's minus teacher's probability
   long long ld, ld_values, ld_indices;
+  float4* partials;   // per row and part: maximum, anchor, sum, whether a class is listed twice
+  long long rows;
   int n, k, values_dtype, indices_wide, parts;
   float c;            // log2(e) / temperature
   double temperature;
@@ -721,36 +727,149 @@ struct Running {
   }
 };
 
-// The student's exponentials are summed over the classes that are NOT kept: the kept ones are taken
-// out of the row in shared memory (each entry writes its number over its class, one that finds
-// another's number there is listed twice; then -inf replaces the numbers). One pass sums relative to
-// the largest value met. One warp evaluates the at most k + 1 terms of the divergence in 64 bits,
-// where the parts that cancel between a student and a teacher that agree do no harm, nor in the
-// gradient's q - p: all but the student's normaliser while the row is still on its way.
-// stats and slopes leave nothing but one exponential per class to the backward pass.
+// Sum of the student's exponentials over the classes that are NOT kept, per row and part: one pass
+// over the logits with a running maximum per thread. A bitmap in shared memory marks the kept classes
+// (one byte test per 8 bf16 elements). Nothing else is done here, so that a dozen small CTAs per SM,
+// each with its own loads in flight, keep HBM busy; the finish kernel is launched at once and works
+// on the kept classes until these sums are there.
 template <typename T>
-__global__ void __launch_bounds__(FT)
-distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
-  constexpr int DT = FT, DW = DT / 32;
+__global__ void __launch_bounds__(ST, 12)
+distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
   constexpr int W = Vec<T>::W;
   using Ord = Order<T>;
-  using Tag = typename std::conditional<sizeof(T) == 4, uint32_t, unsigned short>::type;
-  extern __shared__ __align__(16) uint4 row_smem[];
-  __shared__ int ent_at[ENTRIES];
-  __shared__ double ent_t[ENTRIES], ent_z[ENTRIES], ent_et[ENTRIES], ent_ez[ENTRIES];
-  __shared__ __align__(16) float4 red_run[DW], part_run[MAX_PARTS];
-  __shared__ __align__(8) uint64_t bar_mem;
-  __shared__ int repeated, gave_up;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ uint32_t bitmap[];
+  __shared__ float4 red_run[ST / 32];
+  __shared__ int repeated;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int part = p.parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long r = blockIdx.x / p.parts;
+  const int part = static_cast<int>(blockIdx.x % p.parts);
   const int n = p.n, k = p.k;
   const T* x = logits + r * p.ld;
-  const uint32_t bar = smem_u32(&bar_mem);
-  const StagedRow<T, DT> st(x, n, part, p.parts, row_smem, bar);
-  if (tid == 0) repeated = gave_up = 0;
-  // While the row is on its way the first warp works on the kept entries: their classes, teacher's and
-  // student's logits, both sides' exponentials and sums. The first ENTRIES of them stay in shared memory.
+  const RowLayout<T> lay(x, n);
+  const int per = (lay.vectors + p.parts - 1) / p.parts;
+  const int v0 = min(part * per, lay.vectors), v1 = min(v0 + per, lay.vectors);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + lay.head);
+  constexpr int U = 4;
+  uint4 raw[U];
+  int j0 = v0 + tid;
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+    if (j0 + i * ST < v1) raw[i] = __ldg(xv + j0 + i * ST);
+  // Bit of element e: the part's vectors from bit W on, the row's ends in front of and behind them.
+  const int first = lay.head + v0 * W - W;
+  const int last = part == p.parts - 1 ? n : lay.head + v1 * W;
+  for (int i = tid; i < (last - first + 31) / 32; i += ST) bitmap[i] = 0;
+  if (tid == 0) repeated = 0;
+  __syncthreads();
+  for (int i = tid; i < k; i += ST) {
+    const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+    if (at >= (part == 0 ? 0 : first + W) && at < last) {
+      const int b = at - first;
+      if (atomicOr(&bitmap[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) repeated = 1;
+    }
+  }
+  __syncthreads();
+
+  const float c = p.c;
+  const uint8_t* marks = reinterpret_cast<const uint8_t*>(bitmap);
+  Running run = {-INFINITY, INFINITY, 0.0f};
+  f32x2 acc = 0;
+  auto one_by_one = [&](const uint4& q) {
+    float v[W];
+    unpack(q, v, T());
+#pragma unroll
+    for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
+  };
+  for (; j0 < v1; j0 += U * ST) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = j0 + i * ST;
+      if (j >= v1) break;
+      uint4 q = raw[i];
+      const int b = (j - v0 + 1) * W;
+      const uint32_t mark = (marks[b >> 3] >> (b & 7)) & ((1u << W) - 1u);
+      if (mark) {
+        float v[W];
+        unpack(q, v, T());
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (mark >> e & 1) v[e] = -INFINITY;
+        q = pack(v, T());
+      }
+      const float top = Ord::value_of_largest(Ord::largest(Ord::kLow, q));
+      if (!(top <= run.m)) {  // NaN too
+        if (!(fabsf(top) < FAR) || run.far()) {
+          // The beginning, infinities, NaN, masks' values.
+          float s0, s1;
+          f2_unpack(acc, s0, s1);
+          run.s += s0 + s1;
+          acc = 0;
+          run.raise(top, c);
+          if (!run.far()) acc = exponentials<T>(q, c, run.a);
+          else if (top != -INFINITY) one_by_one(q);
+          continue;
+        }
+        const float a = -top * c;
+        const float f = exp2_approx(a - run.a);
+        acc = f2_mul(acc, f2_pack(f, f));
+        run.s *= f;
+        run.m = top;
+        run.a = a;
+      } else if (run.far()) {
+        if (run.m > -INFINITY) one_by_one(q);
+        continue;
+      }
+      acc = f2_add(acc, exponentials<T>(q, c, run.a));
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (j0 + (U + i) * ST < v1) raw[i] = __ldg(xv + j0 + (U + i) * ST);
+  }
+  float s0, s1;
+  f2_unpack(acc, s0, s1);
+  run.s += s0 + s1;
+  const int edges = (part == 0 ? lay.head : 0) + (part == p.parts - 1 ? lay.tail : 0);
+  if (tid < edges) {
+    const int at = part == 0 && tid < lay.head ? tid : n - lay.tail + (tid - (part == 0 ? lay.head : 0));
+    const int b = at - first;
+    const float v = bitmap[b >> 5] >> (b & 31) & 1 ? -INFINITY : to_float(x[at]);
+    run.raise(v, c);
+    if (!(v == -INFINITY)) run.s += run.of(v, c);
+  }
+  const float m = Order<float>::value(__reduce_max_sync(0xffffffffu, Order<float>::key(__float_as_uint(run.m))));
+  if (m > run.m) run.raise(m, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
+  if (lane == 0) red_run[warp] = make_float4(run.m, run.a, run.s, 0.0f);
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 1; i < ST / 32; ++i) run.join(red_run[i].x, red_run[i].y, red_run[i].z, c);
+    p.partials[blockIdx.x] = make_float4(run.m, run.a, run.s, __int_as_float(repeated));
+  }
+}
+
+// One warp per row evaluates the at most k + 1 terms of the divergence in 64 bits, where the parts
+// that cancel between a student and a teacher that agree do no harm, nor in the gradient's q - p: all
+// but the student's normaliser before the sums over the other classes are waited for. stats and slopes
+// leave nothing but one exponential per class to the backward pass. The first ENTRIES kept classes
+// stay in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(ST)
+distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
+  constexpr int ROWS = ST / 32;
+  __shared__ int at_smem[ROWS][ENTRIES];
+  __shared__ double t_smem[ROWS][ENTRIES], z_smem[ROWS][ENTRIES];
+  __shared__ double et_smem[ROWS][ENTRIES], ez_smem[ROWS][ENTRIES];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long r = static_cast<long long>(blockIdx.x) * ROWS + warp;
+  if (r >= p.rows) return;
+  const int n = p.n, k = p.k;
+  const T* x = logits + r * p.ld;
+  int* ent_at = at_smem[warp];
+  double *ent_t = t_smem[warp], *ent_z = z_smem[warp], *ent_et = et_smem[warp], *ent_ez = ez_smem[warp];
+  const float c = p.c;
   const double inv_t = 1.0 / p.temperature;
   auto load_entry = [&](int i, double& t, double& z) {
     const int at = load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
@@ -761,14 +880,13 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     }
     return at;
   };
-  if (tid < min(k, ENTRIES)) {
+  for (int i = lane; i < min(k, ENTRIES); i += 32) {
     double t, z;
-    ent_at[tid] = load_entry(tid, t, z);
-    ent_t[tid] = t;
-    ent_z[tid] = z;
+    ent_at[i] = load_entry(i, t, z);
+    ent_t[i] = t;
+    ent_z[i] = z;
   }
-  const float c = p.c;
-  __syncthreads();
+  __syncwarp();
   auto class_at = [&](int i) {
     return i < ENTRIES ? ent_at[i] : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
   };
@@ -783,11 +901,10 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     return v;
   };
   // Natural-log units in 64 bits, maxima and sums kept apart (a maximum of the size of a mask's value
-  // would swallow the logarithm of its sum). A class that is listed twice is sorted out later, with
-  // everything here done again.
-  const double tr = p.rest && warp == 0 ? static_cast<double>(p.rest[r]) : -INFINITY;
+  // would swallow the logarithm of its sum).
+  const double tr = p.rest ? static_cast<double>(p.rest[r]) : -INFINITY;
   double t_max, z_max, t_sum, z_sum, t_inv, t_log, fixed_loss, mass;
-  bool silent;
+  bool silent, repeated = false;
   auto part_of = [](double v, double top_value) { return v == -INFINITY ? 0.0 : exp(v - top_value); };
   auto entry = [&](int i, double& t, double& z) {  // teacher's and student's logit; false: left out
     const int at = class_at(i);
@@ -843,111 +960,30 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     fixed_loss = warp_sum(fixed_loss);
     mass = warp_sum(mass);
   };
-  if (warp == 0 && part == 0) work_on_entries();
-  if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
-  Tag* tags = reinterpret_cast<Tag*>(row_smem);
-  const int base = st.v0 * W - st.off, span = (st.v1 - st.v0) * W;
-  auto here = [&](int i) {  // place in this part of the row, -1: none
-    const int at = class_at(i);
-    return at >= 0 && at >= base && at - base < span ? at - base : -1;
-  };
-  for (int i = tid; i < k; i += DT) {
-    const int at = here(i);
-    if (at >= 0) tags[at] = static_cast<Tag>(i);
-  }
-  __syncthreads();
-  for (int i = tid; i < k; i += DT) {
-    const int at = here(i);
-    if (at >= 0 && tags[at] != static_cast<Tag>(i)) repeated = 1;
-  }
-  __syncthreads();
-  for (int i = tid; i < k; i += DT) {
-    const int at = here(i);
-    if (at >= 0) reinterpret_cast<T*>(row_smem)[at] = from_float<T>(-INFINITY);
-  }
-  __syncthreads();
-
-  // One pass: every thread sums relative to the largest value it has met.
-  const int nv = st.v1 - st.v0;
+  work_on_entries();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Running run = {-INFINITY, INFINITY, 0.0f};
-  {
-    f32x2 acc = 0;
-#pragma unroll 2
-    for (int j = tid; j < nv; j += DT) {
-      const uint4 q = st.row[j];
-      const float top = Ord::value_of_largest(Ord::largest(Ord::kLow, q));
-      if (!(top <= run.m)) {  // NaN too
-        if (!(fabsf(top) < FAR) || run.far()) {
-          // Beginning, infinities, NaN, masks' values: one element at a time.
-          float s0, s1;
-          f2_unpack(acc, s0, s1);
-          run.s += s0 + s1;
-          acc = 0;
-          run.raise(top, c);
-          if (!run.far()) {
-            acc = exponentials<T>(q, c, run.a);
-          } else if (top != -INFINITY) {
-            float v[W];
-            unpack(q, v, T());
-#pragma unroll
-            for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
-          }
-          continue;
-        }
-        const float b = -top * c;
-        const float f = exp2_approx(b - run.a);
-        acc = f2_mul(acc, f2_pack(f, f));
-        run.s *= f;
-        run.m = top;
-        run.a = b;
-      } else if (run.far()) {
-        if (run.m > -INFINITY) {
-          float v[W];
-          unpack(q, v, T());
-#pragma unroll
-          for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
-        }
-        continue;
-      }
-      acc = f2_add(acc, exponentials<T>(q, c, run.a));
-    }
-    float s0, s1;
-    f2_unpack(acc, s0, s1);
-    run.s += s0 + s1;
+  int again = 0;
+  if (lane < p.parts) {
+    const float4 f = p.partials[r * p.parts + lane];
+    run = {f.x, f.y, f.z};
+    again = __float_as_int(f.w);
   }
-  {
-    uint32_t best = __reduce_max_sync(0xffffffffu, Order<float>::key(__float_as_uint(run.m)));
-    const float m = Order<float>::value(best);
-    if (m > run.m) run.raise(m, c);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
-    if (lane == 0) red_run[warp] = make_float4(run.m, run.a, run.s, 0.0f);
-  }
-  __syncthreads();
-  if (warp != 0 && p.parts == 1) return;  // one warp finishes the row
-  run = {red_run[0].x, red_run[0].y, red_run[0].z};
-#pragma unroll
-  for (int i = 1; i < DW; ++i) run.join(red_run[i].x, red_run[i].y, red_run[i].z, c);
-  if (p.parts > 1) {
-    if (tid == 0) {
-      const uint32_t dst = mapa_shared(smem_u32(part_run + part), 0);
-      const int flags = repeated | (gave_up << 1);
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(run.m),
-                   "f"(run.a), "f"(run.s), "f"(__int_as_float(flags))
-                   : "memory");
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, run.m, o);
+    const float a = __shfl_xor_sync(0xffffffffu, run.a, o);
+    const float s = __shfl_xor_sync(0xffffffffu, run.s, o);
+    // Both lanes of a pair add the lower lane's value first: all lanes end with the same bits.
+    if (lane & o) {
+      Running low = {m, a, s};
+      low.join(run.m, run.a, run.s, c);
+      run = low;
+    } else {
+      run.join(m, a, s, c);
     }
-    cluster_sync_all();
-    if (part != 0 || warp != 0) return;
-    run = {part_run[0].x, part_run[0].y, part_run[0].z};
-    int any = __float_as_int(part_run[0].w);
-    for (int i = 1; i < p.parts; ++i) {
-      run.join(part_run[i].x, part_run[i].y, part_run[i].z, c);
-      any |= __float_as_int(part_run[i].w);
-    }
-    if (lane == 0) repeated = any & 1, gave_up = any >> 1;
-    __syncwarp();
   }
-
+  repeated = __any_sync(0xffffffffu, again);
   if (repeated) work_on_entries();  // without the entries of classes listed before
   // The classes not kept: zs * e^zm; fmaf(m, c, a) is what rounding the anchor to fp32 left over.
   const bool some = run.s != 0.0f;
@@ -975,7 +1011,7 @@ distill_fwd_kernel(const T* __restrict__ logits, const DistillParams p) {
     const double q_rest = silent || !some ? 0.0 : e_zm / total;
     if (p_rest != 0.0)
       loss += p_rest * ((tr - t_max - t_log) - (some ? zm - top + log(zs) - log_total : -INFINITY));
-    p.loss[r] = gave_up ? NAN : static_cast<float>(loss * p.temperature * p.temperature);
+    p.loss[r] = static_cast<float>(loss * p.temperature * p.temperature);
     // Gradient of a class that is not kept: q_j (1 - p_rest / q_rest).
     p.stats[r] = make_float2(run.m, some ? static_cast<float>((q_rest - p_rest) / run.s) : 0.0f);
   }
@@ -994,7 +1030,8 @@ distill_bwd_kernel(const T* __restrict__ logits, const void* __restrict__ indice
   constexpr int DT = FT;
   constexpr int W = Vec<T>::W;
   const int tid = threadIdx.x;
-  const long long r = blockIdx.x / parts;
+  // The last rows first: the forward pass read them last, and L2 may still hold some of them.
+  const long long r = (gridDim.x - 1 - blockIdx.x) / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
   const T* x = logits + r * ld;
   T* g = grad + r * ld_grad;
@@ -1106,9 +1143,9 @@ int bad(const char* what) {
 constexpr int kTargetCtas = 296;  // two CTAs per SM
 
 // CTAs per row: enough to give every SM two, as long as each keeps `least` vectors.
-int choose_parts(int64_t rows, int vectors, int least) {
+int choose_parts(int64_t rows, int vectors, int least, int64_t target = kTargetCtas, int most = MAX_PARTS) {
   int parts = 1;
-  while (parts < MAX_PARTS && rows * parts < kTargetCtas && vectors / (2 * parts) >= least) parts *= 2;
+  while (parts < most && rows * parts < target && vectors / (2 * parts) >= least) parts *= 2;
   return parts;
 }
 
@@ -1167,22 +1204,66 @@ extern "C" int vmoe_top_logits(const void* logits, int32_t dtype, int64_t rows, 
   return bad("top_logits: unknown dtype");
 }
 
-extern "C" int64_t vmoe_distill_max_classes(int32_t dtype) { return vmoe_top_logits_max_classes(dtype); }
+extern "C" int64_t vmoe_distill_max_classes(int32_t dtype) { return 1 << 20; }
+
+// Eight small CTAs per SM, as long as each keeps two vectors per thread; and no more than 128 K classes
+// (16 KB of bitmap) per part.
+static int distill_parts(int64_t rows, int64_t n, int32_t dtype) {
+  int parts = choose_parts(rows, static_cast<int>(n / (dtype == 0 ? 4 : 8)), 2 * ST, 4 * kTargetCtas,
+                           MAX_SUM_PARTS);
+  while (parts < MAX_SUM_PARTS && n / parts > (1 << 17)) parts *= 2;
+  return parts;
+}
+
+extern "C" int64_t vmoe_distill_kept_floats(int64_t rows, int64_t n, int64_t k, int32_t dtype) {
+  return (rows * (k + 2) + 3) / 4 * 4 + rows * 4 * distill_parts(rows, n, dtype);
+}
+
+template <typename T>
+static int distill_fwd(const VmoeDistillArgs* a, const DistillParams& p, cudaStream_t stream) {
+  const T* logits = static_cast<const T*>(a->logits);
+  constexpr int W = Vec<T>::W;
+  const size_t smem = ((a->n / W + p.parts - 1) / p.parts + 4) * W / 8 + 8;
+  distill_sums_kernel<T><<<static_cast<unsigned>(a->rows * p.parts), ST, smem, stream>>>(logits, p);
+  const int rc = check_launch();
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr;
+  memset(&attr, 0, sizeof(attr));
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>((a->rows + ST / 32 - 1) / (ST / 32)));
+  cfg.blockDim = dim3(ST);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_finish_kernel<T>, logits, p);
+  if (e != cudaSuccess) {
+    set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+    cudaGetLastError();
+    return -5;
+  }
+  return 0;
+}
 
 extern "C" int vmoe_distill_fwd(const VmoeDistillArgs* a, vmoe_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (a->rows == 0) return 0;
-  if (a->rows < 0 || a->rows > MAX_ROWS || a->n < 1 || a->n > vmoe_distill_max_classes(a->dtype) ||
-      a->k < 1 || a->k > 65535)
+  if (a->rows < 0 || a->rows > MAX_ROWS / MAX_SUM_PARTS || a->n < 1 ||
+      a->n > vmoe_distill_max_classes(a->dtype) || a->k < 1 || a->k > (1 << 20))
     return bad("distill: rows, classes or kept classes out of range");
   if (!(a->temperature > 0.0)) return bad("distill: temperature must be positive");
+  if (reinterpret_cast<uintptr_t>(a->kept) & 15) return bad("distill: kept must be 16-byte aligned");
   DistillParams p;
   p.values = a->values;
   p.indices = a->indices;
   p.rest = a->rest;
   p.loss = a->loss;
-  p.stats = reinterpret_cast<float2*>(a->stats);
-  p.slopes = a->slopes;
+  p.stats = reinterpret_cast<float2*>(a->kept);
+  p.slopes = a->kept + 2 * a->rows;
+  p.partials = reinterpret_cast<float4*>(a->kept + (a->rows * (a->k + 2) + 3) / 4 * 4);
+  p.rows = a->rows;
   p.ld = a->ld;
   p.ld_values = a->ld_values;
   p.ld_indices = a->ld_indices;
@@ -1192,15 +1273,11 @@ extern "C" int vmoe_distill_fwd(const VmoeDistillArgs* a, vmoe_stream_t stream_)
   p.indices_wide = a->indices_wide;
   p.c = static_cast<float>(1.4426950408889634 / a->temperature);
   p.temperature = a->temperature;
-  size_t smem = 0;
-  p.parts = staged_parts(a->rows, a->n, a->dtype == 0 ? 4 : 2, 2 * FT, &smem);
+  p.parts = distill_parts(a->rows, a->n, a->dtype);
   switch (a->dtype) {
-    case 0: return launch_clusters(distill_fwd_kernel<float>, a->rows, p.parts, FT, smem, stream,
-                                   static_cast<const float*>(a->logits), p);
-    case 1: return launch_clusters(distill_fwd_kernel<__nv_bfloat16>, a->rows, p.parts, FT, smem, stream,
-                                   static_cast<const __nv_bfloat16*>(a->logits), p);
-    case 2: return launch_clusters(distill_fwd_kernel<__half>, a->rows, p.parts, FT, smem, stream,
-                                   static_cast<const __half*>(a->logits), p);
+    case 0: return distill_fwd<float>(a, p, stream);
+    case 1: return distill_fwd<__nv_bfloat16>(a, p, stream);
+    case 2: return distill_fwd<__half>(a, p, stream);
   }
   return bad("distill: unknown dtype");
 }
@@ -1224,7 +1301,7 @@ extern "C" int vmoe_distill_bwd(const VmoeDistillArgs* a, const float* d_loss, i
 #define VMOE_DISTILL_BWD(T)                                                                         \
   distill_bwd_kernel<T><<<grid, FT, 0, stream>>>(                                                   \
       static_cast<const T*>(a->logits), a->indices, a->indices_wide, a->ld_indices,                 \
-      reinterpret_cast<const float2*>(a->stats), a->slopes, d_loss, d_loss_stride,                  \
+      reinterpret_cast<const float2*>(a->kept), a->kept + 2 * a->rows, d_loss, d_loss_stride,                  \
       static_cast<T*>(grad), a->ld, ld_grad, static_cast<int>(a->n), static_cast<int>(n_pad),       \
       static_cast<int>(a->k), parts, c, static_cast<float>(a->temperature))
   switch (a->dtype) {

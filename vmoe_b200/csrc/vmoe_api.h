@@ -239,8 +239,8 @@ VMOE_API int vmoe_top_logits(const void* logits, int32_t dtype, int64_t rows, in
 // loss (rows, fp32) = temperature^2 * KL(teacher || student) over the kept classes and, when rest is
 // set, "any other class" as one more outcome; the teacher's distribution is the softmax of
 // values / temperature (and rest). Entries whose index lies outside 0 .. n - 1 are left out, of a
-// class listed twice the first entry counts. stats (rows, 2) and slopes (rows, k), fp32, are kept
-// for the backward pass, which writes grad (rows, ld_grad) = d loss / d logits * d_loss in the
+// class listed twice the first entry counts. kept (vmoe_distill_kept_floats() floats) carries what the
+// backward pass needs; that one writes grad (rows, ld_grad) = d loss / d logits * d_loss in the
 // logits' type; columns n .. n_pad - 1 get zeros. grad rows must have the logits rows' alignment
 // within 16 bytes. d_loss_stride 0: one value for all rows.
 typedef struct VmoeDistillArgs {
@@ -249,8 +249,7 @@ typedef struct VmoeDistillArgs {
   const void* indices;
   const float* rest;  // may be NULL
   float* loss;
-  float* stats;
-  float* slopes;
+  float* kept;
   int64_t rows, n, k;
   int64_t ld, ld_values, ld_indices;  // row strides in elements
   double temperature;
@@ -258,6 +257,7 @@ typedef struct VmoeDistillArgs {
   int32_t indices_wide;               // 0: int32, 1: int64
 } VmoeDistillArgs;
 VMOE_API int64_t vmoe_distill_max_classes(int32_t dtype);
+VMOE_API int64_t vmoe_distill_kept_floats(int64_t rows, int64_t n, int64_t k, int32_t dtype);
 VMOE_API int vmoe_distill_fwd(const VmoeDistillArgs* args, vmoe_stream_t stream);
 VMOE_API int vmoe_distill_bwd(const VmoeDistillArgs* args, const float* d_loss,
                               int64_t d_loss_stride, void* grad, int64_t ld_grad, int64_t n_pad,

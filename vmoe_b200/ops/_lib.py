@@ -98,8 +98,7 @@ class DistillArgs(ctypes.Structure):
   """Mirror of ``VmoeDistillArgs``."""
   _fields_ = [
       ("logits", ctypes.c_void_p), ("values", ctypes.c_void_p), ("indices", ctypes.c_void_p),
-      ("rest", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("stats", ctypes.c_void_p),
-      ("slopes", ctypes.c_void_p),
+      ("rest", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("kept", ctypes.c_void_p),
       ("rows", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
       ("ld", ctypes.c_int64), ("ld_values", ctypes.c_int64), ("ld_indices", ctypes.c_int64),
       ("temperature", ctypes.c_double),
@@ -132,6 +131,8 @@ def lib() -> ctypes.CDLL:
       l.vmoe_distill_max_classes.restype = i64
       l.vmoe_distill_max_classes.argtypes = [i32]
       l.vmoe_top_logits.argtypes = [vp, i32, i64, i64, i64, i64, ctypes.c_double, vp, vp, vp, vp]
+      l.vmoe_distill_kept_floats.restype = i64
+      l.vmoe_distill_kept_floats.argtypes = [i64, i64, i64, i32]
       l.vmoe_distill_fwd.argtypes = [vp, vp]
       l.vmoe_distill_bwd.argtypes = [vp, vp, i64, vp, i64, i64, vp]
       l.vmoe_gated_scratch_bytes.restype = i64

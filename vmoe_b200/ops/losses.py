@@ -169,19 +169,19 @@ class _DistillFn(torch.autograd.Function):
       dev = x.device
       a = _lib.DistillArgs()
       loss = torch.empty(rows, dtype=torch.float32, device=dev)
-      kept = torch.empty((k + 2) * rows, dtype=torch.float32, device=dev)  # stats, slopes
+      lib, code = _lib.lib(), _FLOAT_CODES[x.dtype]
+      kept = torch.empty(lib.vmoe_distill_kept_floats(rows, n, k, code), dtype=torch.float32,
+                         device=dev)
       a.logits, a.values, a.indices = x.data_ptr(), values.data_ptr(), indices.data_ptr()
       if rest is not None:
         a.rest = rest.data_ptr()
-      a.loss, a.stats = loss.data_ptr(), kept.data_ptr()
-      a.slopes = kept.data_ptr() + 8 * rows
+      a.loss, a.kept = loss.data_ptr(), kept.data_ptr()
       a.rows, a.n, a.k, a.temperature = rows, n, k, temperature
       a.ld, a.ld_values, a.ld_indices = _ld(x), _ld(values), _ld(indices)
-      a.dtype, a.values_dtype = _FLOAT_CODES[x.dtype], _FLOAT_CODES[values.dtype]
+      a.dtype, a.values_dtype = code, _FLOAT_CODES[values.dtype]
       a.indices_wide = indices.dtype == torch.int64
-      _lib.check(_lib.lib().vmoe_distill_fwd(ctypes.byref(a), _lib.stream_ptr()),
-                 "vmoe_distill_fwd")
-      _lib.count_launch()
+      _lib.check(lib.vmoe_distill_fwd(ctypes.byref(a), _lib.stream_ptr()), "vmoe_distill_fwd")
+      _lib.count_launch(2)
     ctx.save_for_backward(x, indices, kept)
     ctx.args = a
     return loss
@@ -268,7 +268,7 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
   dev = logits.device
   if values.device != dev or indices.device != dev or (rest is not None and rest.device != dev):
     raise ValueError(f"distill_xent: values, indices and rest must be on {dev} like logits")
-  if _on_kernels(logits, "distill") and values.shape[1] <= 65535:
+  if _on_kernels(logits, "distill") and values.shape[1] <= 1 << 20:
     if values.dtype not in _FLOAT_CODES:
       values = values.float()
     if rest is not None and (rest.dtype != torch.float32 or not rest.is_contiguous()):
