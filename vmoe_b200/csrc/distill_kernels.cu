@@ -179,6 +179,36 @@ __device__ __forceinline__ uint32_t bits_at(const uint4& q, int e) {
   return e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
 }
 
+template <typename T>
+__device__ __forceinline__ uint4 low_vector() {  // -inf everywhere
+  constexpr uint32_t w = Order<T>::kLow;
+  return make_uint4(w, w, w, w);
+}
+
+// -inf in place of the elements whose bit is set in `mark`.
+__device__ __forceinline__ void mask_vector(uint4& q, uint32_t mark, float) {
+  if (mark & 1) q.x = 0xff800000u;
+  if (mark & 2) q.y = 0xff800000u;
+  if (mark & 4) q.z = 0xff800000u;
+  if (mark & 8) q.w = 0xff800000u;
+}
+template <typename T>
+__device__ __forceinline__ void mask_vector(uint4& q, uint32_t mark, T) {
+  // Four bits to the tops of four bytes, each top to 16 bits.
+  const uint32_t lo = ((mark & 15u) * 0x10204080u) & 0x80808080u;
+  const uint32_t hi = (((mark >> 4) & 15u) * 0x10204080u) & 0x80808080u;
+  uint32_t m[4];  // selector 8 + i: the sign of byte i, eight times
+  asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m[0]) : "r"(lo));
+  asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m[1]) : "r"(lo));
+  asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m[2]) : "r"(hi));
+  asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m[3]) : "r"(hi));
+  constexpr uint32_t low = Order<T>::kLow;
+  q.x = (q.x & ~m[0]) | (low & m[0]);
+  q.y = (q.y & ~m[1]) | (low & m[1]);
+  q.z = (q.z & ~m[2]) | (low & m[2]);
+  q.w = (q.w & ~m[3]) | (low & m[3]);
+}
+
 // Sum of 2^(x c + a) over a vector, as two partial sums.
 template <typename T>
 __device__ __forceinline__ f32x2 exponentials(const uint4& q, float c, float a) {
@@ -332,11 +362,12 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   extern __shared__ __align__(16) uint4 row_smem[];
   __shared__ __align__(16) u64 cand[TOP_CAP];
   __shared__ __align__(16) u64 sorted[TOP_CAP];
+  __shared__ __align__(16) uint32_t brief[TOP_CAP];
   __shared__ uint32_t red_u[DT / 32];
   __shared__ float red_f[DT / 32];
   __shared__ float2 part_rest[MAX_PARTS];
   __shared__ __align__(8) uint64_t bar_mem;
-  __shared__ int count, hot_count, gave_up;
+  __shared__ int count, hot_count, gave_up, too_wide;
   __shared__ uint2 red_range[DT / 32];
   __shared__ u64 part_bound[MAX_PARTS];
   __shared__ int list_length[MAX_PARTS];
@@ -349,7 +380,7 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   const StagedRow<T, DT> st(x, n, part, parts, row_smem, bar);
   const int nv = st.v1 - st.v0;
   const int mine = min(k, st.elements());  // entries this part can contribute
-  if (tid == 0) count = hot_count = gave_up = 0, odd_sum = 0;
+  if (tid == 0) count = hot_count = gave_up = too_wide = 0, odd_sum = 0;
   __syncthreads();
   if (!mbar_wait(bar, 0, &gave_up, nullptr, 0)) gave_up = 1;
 
@@ -398,11 +429,21 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     const bool near = fabsf(m) < FAR;
     const float anchor = near ? -m * c : 0.0f;
     f32x2 acc = 0;
-    u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-31
+    u64 odd = 0;  // what shares a vector with a candidate, in units of 2^-28
     // Candidates of the vector j (none if `has` is false); all lanes of a warp take part.
     auto take_apart = [&](bool has, int j) {
       uint32_t hits = 0;
-      if (has) {
+      if (has && attempt == 0 && near) {
+        // An ordinary bound: whatever is not below it is a candidate (padding is -inf).
+        float v[W], below = 0.0f;
+        unpack(st.row[j], v, T());
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (v[e] < m) below += exp2_approx(fmaf(v[e], c, anchor));
+          else hits |= 1u << e;
+        }
+        odd += __float2uint_rn(below * 0x1p28f);
+      } else if (has) {
         const uint4 q = st.row[j];
 #pragma unroll
         for (int e = 0; e < W; ++e) {
@@ -410,20 +451,25 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
           const int at = st.position(j, e);
           if (static_cast<unsigned>(at) >= static_cast<unsigned>(n)) continue;
           if (taken(key, at)) hits |= 1u << e;
-          else if (near) odd += __float2uint_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p31f);
+          else if (near) odd += __float2uint_rn(exp2_approx(fmaf(Ord::value(key), c, anchor)) * 0x1p28f);
         }
       }
       int pos = claim(&count, __popc(hits));
       for (; hits && pos < TOP_CAP; hits &= hits - 1, ++pos) {
         const int at = st.position(j, __ffs(hits) - 1);
-        cand[pos] = (static_cast<u64>(Ord::key(st.bits(at))) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+        const uint32_t key = Ord::key(st.bits(at));
+        cand[pos] = (static_cast<u64>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(at));
+        if (sizeof(T) == 2) {  // order in 32 bits, where key and position fit
+          brief[pos] = ((key - bound) << 20) | (0xfffffu - static_cast<uint32_t>(at));
+          if (key - bound >= 4096u) too_wide = 1;
+        }
       }
     };
     if (attempt == 0) {
       u64 mine_hot = 0;  // bit i: vector tid + i DT (at most MAX_PART_BYTES / 16 / DT = 44 of them)
-      int j = tid;
+      int i = 0;
 #pragma unroll 2
-      for (int i = 0; j < nv; j += DT, ++i) {
+      for (int j = tid; j < nv; j += DT, ++i) {
         const uint4 q = st.row[j];
         const f32x2 sum = exponentials<T>(q, c, anchor);
         if (Ord::all_below(Ord::largest(Ord::kLow, q), m)) acc = f2_add(acc, sum);
@@ -502,25 +548,44 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
 
   // Rank of every candidate = number of larger ones (all are different: the position is part). Four
   // threads count for one candidate.
-  if (tid < 8 && found + tid < TOP_CAP) cand[found + tid] = 0;  // the list is read in blocks of 8
+  if (tid < 8 && found + tid < TOP_CAP) cand[found + tid] = brief[found + tid] = 0;  // read in blocks
   __syncthreads();
-  for (int q0 = 0; q0 < found; q0 += DT / 4) {
-    const int q = q0 + (tid >> 2);
-    const u64 me = q < found ? cand[q] : ~0ull;
-    int rank = 0;
-    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
-#pragma unroll 2
-    for (int j = tid & 3; j < (found + 1) / 2; j += 4) {
-      const ulonglong2 two = pairs[j];
-      rank += (two.x > me ? 1 : 0) + (two.y > me ? 1 : 0);
+  auto rank_all = [&](auto* list, auto count_larger) {
+    for (int q0 = 0; q0 < found; q0 += DT / 4) {
+      const int q = q0 + (tid >> 2);
+      if (q0 + ((tid & ~31) >> 2) >= found) break;  // whole warps
+      int rank = count_larger(list[q < found ? q : 0]);
+      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+      if (q < found && (tid & 3) == 0) sorted[rank] = cand[q];
     }
-    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-    if (q < found && (tid & 3) == 0) sorted[rank] = me;
+  };
+  if (sizeof(T) == 2 && !too_wide && n <= (1 << 20)) {
+    rank_all(brief, [&](uint32_t me) {
+      int rank = 0;
+      const uint4* four = reinterpret_cast<const uint4*>(brief);
+#pragma unroll 2
+      for (int j = tid & 3; j < (found + 3) / 4; j += 4) {
+        const uint4 v = four[j];
+        rank += (v.x > me ? 1 : 0) + (v.y > me ? 1 : 0) + (v.z > me ? 1 : 0) + (v.w > me ? 1 : 0);
+      }
+      return rank;
+    });
+  } else {
+    rank_all(cand, [&](u64 me) {
+      int rank = 0;
+      const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(cand);
+#pragma unroll 2
+      for (int j = tid & 3; j < (found + 1) / 2; j += 4) {
+        const ulonglong2 two = pairs[j];
+        rank += (two.x > me ? 1 : 0) + (two.y > me ? 1 : 0);
+      }
+      return rank;
+    });
   }
   s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
   if (fabsf(m) < FAR)  // the last factor takes the rounding of m c back
-    s = (s + static_cast<float>(odd_sum) * 0x1p-31f) * exp2_approx(-fmaf(m, c, -m * c));
+    s = (s + static_cast<float>(odd_sum) * 0x1p-28f) * exp2_approx(-fmaf(m, c, -m * c));
   // Adds values (each thread's own, through `each`) whose largest key is `key` to the sum; none of
   // them lies below what is in the sum already.
   auto add_at = [&](uint32_t key, auto each) {
@@ -750,12 +815,24 @@ distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
   const int per = (lay.vectors + p.parts - 1) / p.parts;
   const int v0 = min(part * per, lay.vectors), v1 = min(v0 + per, lay.vectors);
   const uint4* xv = reinterpret_cast<const uint4*>(x + lay.head);
+  // Four vectors per thread and step; -inf past the end in the last, partial step.
   constexpr int U = 4;
   uint4 raw[U];
-  int j0 = v0 + tid;
+  const int mine = v1 - v0 - tid;  // vectors from this thread's first one on
+  const int full = (v1 - v0) / (U * ST);
+  const uint4* next = xv + v0 + tid;
+  auto fetch = [&](int step) {
+    if (step < full) {
 #pragma unroll
-  for (int i = 0; i < U; ++i)
-    if (j0 + i * ST < v1) raw[i] = __ldg(xv + j0 + i * ST);
+      for (int i = 0; i < U; ++i) raw[i] = __ldg(next + i * ST);
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        raw[i] = (step * U + i) * ST < mine ? __ldg(next + i * ST) : low_vector<T>();
+    }
+    next += U * ST;
+  };
+  fetch(0);
   // Bit of element e: the part's vectors from bit W on, the row's ends in front of and behind them.
   const int first = lay.head + v0 * W - W;
   const int last = part == p.parts - 1 ? n : lay.head + v1 * W;
@@ -772,59 +849,45 @@ distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
   __syncthreads();
 
   const float c = p.c;
-  const uint8_t* marks = reinterpret_cast<const uint8_t*>(bitmap);
   Running run = {-INFINITY, INFINITY, 0.0f};
+  float limit = NAN;  // the maximum so far while it is an ordinary number: nothing is <= NaN
   f32x2 acc = 0;
-  auto one_by_one = [&](const uint4& q) {
-    float v[W];
-    unpack(q, v, T());
-#pragma unroll
-    for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
-  };
-  for (; j0 < v1; j0 += U * ST) {
+  // Marks of this thread's vectors: a byte each, or half a byte with four elements to a vector.
+  const uint8_t* mark_at = reinterpret_cast<const uint8_t*>(bitmap) + (W == 8 ? tid + 1 : (tid + 1) >> 1);
+  const int mark_shift = W == 8 ? 0 : ((tid + 1) & 1) * 4;
+  for (int step = 0; step * U * ST < mine; ++step) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int j = j0 + i * ST;
-      if (j >= v1) break;
-      uint4 q = raw[i];
-      const int b = (j - v0 + 1) * W;
-      const uint32_t mark = (marks[b >> 3] >> (b & 7)) & ((1u << W) - 1u);
-      if (mark) {
-        float v[W];
-        unpack(q, v, T());
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          if (mark >> e & 1) v[e] = -INFINITY;
-        q = pack(v, T());
-      }
-      const float top = Ord::value_of_largest(Ord::largest(Ord::kLow, q));
-      if (!(top <= run.m)) {  // NaN too
-        if (!(fabsf(top) < FAR) || run.far()) {
-          // The beginning, infinities, NaN, masks' values.
-          float s0, s1;
-          f2_unpack(acc, s0, s1);
-          run.s += s0 + s1;
-          acc = 0;
-          run.raise(top, c);
-          if (!run.far()) acc = exponentials<T>(q, c, run.a);
-          else if (top != -INFINITY) one_by_one(q);
-          continue;
-        }
-        const float a = -top * c;
-        const float f = exp2_approx(a - run.a);
-        acc = f2_mul(acc, f2_pack(f, f));
-        run.s *= f;
-        run.m = top;
-        run.a = a;
-      } else if (run.far()) {
-        if (run.m > -INFINITY) one_by_one(q);
-        continue;
-      }
-      acc = f2_add(acc, exponentials<T>(q, c, run.a));
+      if (step >= full && (step * U + i) * ST >= mine) break;
+      const uint32_t mark = (mark_at[i * ST * W / 8] >> mark_shift) & ((1u << W) - 1u);
+      if (mark) mask_vector(raw[i], mark, T());
     }
+    mark_at += U * ST * W / 8;
+    uint32_t most = Ord::largest(Ord::kLow, raw[0]);
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (j0 + (U + i) * ST < v1) raw[i] = __ldg(xv + j0 + (U + i) * ST);
+    for (int i = 1; i < U; ++i) most = Ord::largest(most, raw[i]);
+    const float top = Ord::value_of_largest(most);
+    if (!(top <= limit)) {  // NaN too
+      float s0, s1;
+      f2_unpack(acc, s0, s1);
+      run.s += s0 + s1;
+      acc = 0;
+      run.raise(top, c);
+      limit = run.far() ? NAN : run.m;
+    }
+    if (!run.far()) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) acc = f2_add(acc, exponentials<T>(raw[i], c, run.a));
+    } else if (run.m > -INFINITY || top != -INFINITY) {  // infinities, NaN, masks' values
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        float v[W];
+        unpack(raw[i], v, T());
+#pragma unroll
+        for (int e = 0; e < W; ++e) run.s += exp2_approx((v[e] - run.m) * c);
+      }
+    }
+    fetch(step + 1);
   }
   float s0, s1;
   f2_unpack(acc, s0, s1);
