@@ -150,6 +150,11 @@ SHAPES = [
     (1, 777, 320, 3416, None, True, True),
     (8, 300, 192, 776, None, True, False),
     (1, 2600, 128, 1024, 264, True, True),
+    (8, 52, 128, 344, None, True, True),
+    (3, 64, 192, 264, 136, True, False),
+    (5, 100, 64, 72, None, False, True),
+    (1, 1285, 256, 680, 1280, True, True),
+    (1, 400, 520, 2048, None, True, False),
 ]
 
 

@@ -7,11 +7,15 @@
 //
 // Both are persistent warp-specialised GEMMs (TMA -> 128B-swizzled shared memory -> tcgen05.mma ->
 // TMEM -> epilogue warps), with one CTA per 128-row tile or CTA pairs on 256-row tiles, like the
-// plain GEMM of this library. Forward: the 256 accumulator columns of a tile are 128 gate columns
-// and the 128 up columns of the same hidden units, so a thread of the epilogue finds both factors
-// of its products in its own TMEM lane; in a CTA pair the even CTA stages the gate's rows of the
-// weights and the odd CTA the up projection's. Backward: the saved factors come in by TMA, one
-// 32 x 32 tile ahead of their use, and the epilogue is two products.
+// plain GEMM of this library. Forward: half of a tile's accumulator columns are gate columns and half
+// the up columns of the same hidden units, so a thread of the epilogue finds both factors of its
+// products in its own TMEM lane; in a CTA pair the even CTA stages the gate's rows of the weights
+// and the odd CTA the up projection's. Backward: the saved factors come in by TMA, one 32 x 32 tile
+// ahead of their use, and the epilogue is two products.
+//
+// The same kernel with a plain epilogue does the block's other two products with rows of x (output
+// projection, dx) where the plain GEMM's 256-column tiles would leave SMs idle: tiles are 256, 128 or
+// 64 accumulator columns wide, and the host takes the shape with the shortest estimate.
 //
 // Saving a and s (rounded once from fp32) instead of g and u leaves one rounding in each factor and
 // no transcendental function in the backward pass; the traffic is the same. dg and du are rounded
@@ -36,24 +40,19 @@ int make_bf16_map(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t ro
 namespace {
 
 constexpr int BM = 128;
-constexpr int BN = 256;
-constexpr int HALF = BN / 2;
 constexpr int BK = 64;
 constexpr int UMMA_K = 16;
-constexpr int A_BYTES = BM * BK * 2;        // 16 KiB
-constexpr int B_BYTES = BN * BK * 2;        // 32 KiB
+constexpr int ROW_BYTES = BK * 2;           // one row of a K-major operand in a stage
 constexpr int CHUNK_BYTES = 64 * BK * 2;    // one 64 x 64 MN-major box
-constexpr int STAGES = 3;                   // one CTA: 48 KiB per stage
-constexpr int STAGES_PAIR = 5;              // pairs stage half of B per CTA: 32 KiB per stage
-constexpr int TMEM_COLS = 512;
+constexpr int MAX_STAGES = 10;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TILE_BYTES = 32 * 32 * 2;     // one staging tile: 32 rows of 64 bytes, 64B swizzle
 constexpr int EPI_TILES = 4;                // per epilogue warp
-constexpr int PIPE_BYTES = STAGES_PAIR * (A_BYTES + B_BYTES / 2);
-constexpr int SMEM_BYTES = PIPE_BYTES + EPI_WARPS * EPI_TILES * TILE_BYTES + 1024 + 256;
-static_assert(STAGES * (A_BYTES + B_BYTES) <= PIPE_BYTES, "both modes share one budget");
+constexpr int PIPE_BYTES = 160 * 1024;      // stages of A rows and B rows, as many as fit
+constexpr int SMEM_BYTES = PIPE_BYTES + EPI_WARPS * EPI_TILES * TILE_BYTES + 1024 + 320;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+static_assert((2 * MAX_STAGES + 4 + EPI_WARPS) * 8 + 8 <= 320, "room for the barriers");
 
 // Tiled copies with four coordinates (column, factor, row, expert).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int c0,
@@ -103,6 +102,9 @@ struct GatedParams {
   int rows, k, m, batch;
   int act;            // 0 GELU (tanh form), 1 SiLU
   int save;           // forward: write a and s
+  int a_box, stages;  // rows of A per load (fewer than 128 when there are fewer), pipeline stages
+  const __nv_bfloat16* residual;  // plain: (E, rows, m) with strides, or NULL
+  long long ldr, r_batch_stride;
 };
 
 }  // namespace
@@ -115,7 +117,9 @@ namespace {
 
 // MODE 0: forward. A = x (rows x k), B = w_in as (k, m, 2 E), both K-major.
 // MODE 1: backward. A = dy (rows x k, K-major), B = w_out (m contiguous: MN-major).
-template <bool PAIR, int MODE>
+// MODE 2 / 3: plain A B^T + bias + residual, B K-major / MN-major.
+// BN: accumulator columns of a tile.
+template <bool PAIR, int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
              const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_s,
@@ -123,21 +127,28 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  constexpr int NSTAGE = PAIR ? STAGES_PAIR : STAGES;
-  constexpr int BSTAGE = PAIR ? B_BYTES / 2 : B_BYTES;
+  constexpr int HALF = BN / 2;
+  constexpr bool B_MN = MODE == 1 || MODE == 3;
+  constexpr int B_ROWS = PAIR ? HALF : BN;  // rows (columns of the result) of B this CTA stages
+  constexpr int BSTAGE = B_ROWS * ROW_BYTES;
+  constexpr int TMEM_COLS = 2 * BN;
   constexpr int TM = PAIR ? 2 * BM : BM;
-  constexpr int TN = MODE == 0 ? HALF : BN;  // hidden units per tile
+  constexpr int TN = MODE == 0 ? HALF : BN;  // columns of the result per tile
+  static_assert(!B_MN || B_ROWS % 64 == 0, "MN-major boxes are 64 columns wide");
+  const int nstage = p.stages;
+  // Rows of A that are not loaded keep what the stage held before: their results are not stored.
+  const int a_stage = max(p.a_box, 8) * ROW_BYTES;
   uint8_t* sA = smem;
-  uint8_t* sB = smem + NSTAGE * A_BYTES;
+  uint8_t* sB = smem + nstage * a_stage;
   uint8_t* sEpi = smem + PIPE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + EPI_WARPS * EPI_TILES * TILE_BYTES);
-  // full[NSTAGE], empty[NSTAGE], accumulator full[2], accumulator empty[2], epilogue input[8]
+  // full[stages], empty[stages], accumulator full[2], accumulator empty[2], epilogue input[8]
   const uint32_t bar_full = smem_u32(bars);
-  const uint32_t bar_empty = smem_u32(bars + NSTAGE);
-  const uint32_t bar_tfull = smem_u32(bars + 2 * NSTAGE);
-  const uint32_t bar_tempty = smem_u32(bars + 2 * NSTAGE + 2);
-  const uint32_t bar_in = smem_u32(bars + 2 * NSTAGE + 4);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NSTAGE + 4 + EPI_WARPS);
+  const uint32_t bar_empty = smem_u32(bars + nstage);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * nstage);
+  const uint32_t bar_tempty = smem_u32(bars + 2 * nstage + 2);
+  const uint32_t bar_in = smem_u32(bars + 2 * nstage + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * nstage + 4 + EPI_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int cta = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -147,7 +158,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < NSTAGE; ++s) {
+    for (int s = 0; s < nstage; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
@@ -205,11 +216,11 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           }
           const uint32_t full = full_base + 8 * stage;
           if (!PAIR) {
-            mbar_expect_tx(full, A_BYTES + BSTAGE);
+            mbar_expect_tx(full, a_stage + BSTAGE);
           } else if (rank == 0) {
-            mbar_expect_tx(bar_full + 8 * stage, 2 * (A_BYTES + BSTAGE));
+            mbar_expect_tx(bar_full + 8 * stage, 2 * (a_stage + BSTAGE));
           }
-          const uint32_t a_dst = smem_u32(sA + stage * A_BYTES);
+          const uint32_t a_dst = smem_u32(sA + stage * a_stage);
           const uint32_t b_dst = smem_u32(sB + stage * BSTAGE);
           const int k0 = kt * BK;
           auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
@@ -225,15 +236,18 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
               load(b_dst, &map_b, k0, nt * TN, 2 * b + static_cast<int>(rank));
             } else {
               load(b_dst, &map_b, k0, nt * TN, 2 * b);
-              load(b_dst + B_BYTES / 2, &map_b, k0, nt * TN, 2 * b + 1);
+              load(b_dst + BSTAGE / 2, &map_b, k0, nt * TN, 2 * b + 1);
             }
           } else {
             const int n0 = nt * TN + static_cast<int>(rank) * HALF;
+            if (!B_MN) {
+              load(b_dst, &map_b, k0, n0, b);
+            } else {
 #pragma unroll
-            for (int j = 0; j < (PAIR ? HALF : BN) / 64; ++j)
-              load(b_dst + j * CHUNK_BYTES, &map_b, n0 + 64 * j, k0, b);
+              for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * CHUNK_BYTES, &map_b, n0 + 64 * j, k0, b);
+            }
           }
-          if (++stage == NSTAGE) {
+          if (++stage == nstage) {
             stage = 0;
             phase ^= 1;
           }
@@ -247,8 +261,8 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = umma_idesc_bf16(TM, BN, 0, MODE);
-      const uint32_t b_lbo = MODE ? CHUNK_BYTES : 16, b_step = MODE ? 2048 : 32;
+      const uint32_t idesc = umma_idesc_bf16(TM, BN, 0, B_MN ? 1 : 0);
+      const uint32_t b_lbo = B_MN ? CHUNK_BYTES : 16, b_step = B_MN ? 2048 : 32;
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -265,7 +279,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + stage * A_BYTES);
+          const uint32_t a_addr = smem_u32(sA + stage * a_stage);
           const uint32_t b_addr = smem_u32(sB + stage * BSTAGE);
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k) {
@@ -282,7 +296,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           } else {
             umma_commit(bar_empty + 8 * stage);
           }
-          if (++stage == NSTAGE) {
+          if (++stage == nstage) {
             stage = 0;
             phase ^= 1;
           }
@@ -303,7 +317,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     uint8_t* tiles = sEpi + ew * EPI_TILES * TILE_BYTES;
     const uint32_t st_row = static_cast<uint32_t>(lane) * 64u;
     const uint32_t st_xor = (static_cast<uint32_t>(lane) >> 1) & 3u;
-    constexpr int CHUNKS = TN / 32 / 2;  // 32-column chunks per warp and tile
+    constexpr int CHUNKS = TN / 32;  // 32-column chunks of a tile, shared by two warps per quadrant
     const uint32_t in_bar = bar_in + 8 * ew;
     const uint32_t tempty_base = PAIR ? mapa_shared(bar_tempty, 0) : bar_tempty;
     uint32_t in_phase = 0;
@@ -335,7 +349,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           tma_load_4d(smem_u32(tiles + 3 * TILE_BYTES), &map_s, in_bar, col0, 1, row0, b);
         }
       };
-      if (MODE == 1 && n0 + half * CHUNKS * 32 < p.m) fetch(n0 + half * CHUNKS * 32);
+      if (MODE == 1 && n0 + half * 32 < p.m) fetch(n0 + half * 32);
       const bool got = mbar_wait(bar_tfull + 8 * slot, use & 1, abort_flag, nullptr, 0);
       if (!__all_sync(0xffffffffu, got)) {
         ok = false;
@@ -343,7 +357,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int c = half * CHUNKS; c < half * CHUNKS + CHUNKS; ++c) {
+      for (int c = half; c < CHUNKS; c += 2) {
         const int col0 = n0 + c * 32;
         if (col0 >= p.m) break;
         const uint32_t acc =
@@ -426,6 +440,62 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
+        } else if (MODE >= 2) {
+          uint32_t r[32];
+          tmem_ld_32x32(acc, r);
+          const int row = row0 + lane;
+          const __nv_bfloat16* res = p.residual && row < p.rows
+                                         ? p.residual + b * p.r_batch_stride + row * p.ldr + col0
+                                         : nullptr;
+          uint4 rq[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // m is a multiple of 8
+            rq[i] = make_uint4(0, 0, 0, 0);
+            if (res && col0 + 8 * i < p.m) rq[i] = __ldg(reinterpret_cast<const uint4*>(res) + i);
+          }
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w[4] = {rq[i].x, rq[i].y, rq[i].z, rq[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack_bf16x2(w[j]);
+              v[8 * i + 2 * j] = __uint_as_float(r[8 * i + 2 * j]) + f.x;
+              v[8 * i + 2 * j + 1] = __uint_as_float(r[8 * i + 2 * j + 1]) + f.y;
+            }
+          }
+          if (p.bias) {
+            const long long at = static_cast<long long>(b) * p.m + col0;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              if (col0 + i >= p.m) break;
+              float4 f;
+              if (p.bias_bf16) {
+                const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.bias) + at + i));
+                const float2 f0 = unpack_bf16x2(q.x), f1 = unpack_bf16x2(q.y);
+                f = make_float4(f0.x, f0.y, f1.x, f1.y);
+              } else {
+                f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + at + i));
+              }
+              v[i] += f.x;
+              v[i + 1] += f.y;
+              v[i + 2] += f.z;
+              v[i + 3] += f.w;
+            }
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          stage_row(tiles, w);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&map_h, smem_u32(tiles), col0, row0, b);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
         } else {
           uint32_t r[32];
           tmem_ld_32x32(acc, r);
@@ -444,7 +514,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           }
           tmem_ld_wait();
           __syncwarp();
-          if (c + 1 < half * CHUNKS + CHUNKS && col0 + 32 < p.m) fetch(col0 + 32);
+          if (c + 2 < CHUNKS && col0 + 64 < p.m) fetch(col0 + 64);
           uint32_t wg[16], wu[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -654,6 +724,26 @@ struct DeviceInfo {
   int sms, pairs;
 };
 
+// Tile shapes: 128 rows and one CTA, or 256 rows and a CTA pair, times accumulator columns.
+struct Shape {
+  bool pair;
+  int bn;
+};
+constexpr Shape SHAPES[4] = {{true, 256}, {true, 128}, {false, 128}, {false, 64}};
+
+using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
+                        const CUtensorMap, const GatedParams);
+template <int MODE>
+Kernel kernel_in(const Shape& s) {
+  if (!s.pair) return s.bn == 128 ? gated_kernel<false, MODE, 128> : gated_kernel<false, MODE, 64>;
+  if (s.bn == 128) return gated_kernel<true, MODE, 128>;
+  if constexpr (MODE < 2) return gated_kernel<true, MODE, 256>;
+  return nullptr;  // the library's plain GEMM
+}
+Kernel kernel_of(int mode, const Shape& s) {
+  return mode == 0 ? kernel_in<0>(s) : mode == 1 ? kernel_in<1>(s) : mode == 2 ? kernel_in<2>(s) : kernel_in<3>(s);
+}
+
 // Per-device set-up (shared-memory limits, resident CTA pairs), done once per device.
 int device_info(DeviceInfo* out) {
   constexpr int MAX_DEVICES = 64;
@@ -665,12 +755,11 @@ int device_info(DeviceInfo* out) {
   if (!ready[dev]) {
     DeviceInfo d = {0, 0};
     e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-    const void* kernels[4] = {reinterpret_cast<const void*>(gated_kernel<false, 0>),
-                              reinterpret_cast<const void*>(gated_kernel<false, 1>),
-                              reinterpret_cast<const void*>(gated_kernel<true, 0>),
-                              reinterpret_cast<const void*>(gated_kernel<true, 1>)};
-    for (int i = 0; i < 4 && e == cudaSuccess; ++i)
-      e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    for (int mode = 0; mode < 4; ++mode)
+      for (const Shape& shape : SHAPES)
+        if (e == cudaSuccess && kernel_of(mode, shape))
+          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel_of(mode, shape)),
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) {
       set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
       return -4;
@@ -688,7 +777,7 @@ int device_info(DeviceInfo* out) {
     cfg.dynamicSmemBytes = SMEM_BYTES;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&d.pairs, gated_kernel<true, 0>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&d.pairs, gated_kernel<true, 0, 256>, &cfg) != cudaSuccess) {
       cudaGetLastError();
       d.pairs = 0;
     }
@@ -699,15 +788,56 @@ int device_info(DeviceInfo* out) {
   return 0;
 }
 
-template <int MODE>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh, const CUtensorMap& ms,
-           const CUtensorMap& md, const GatedParams& p, const DeviceInfo& info, bool pair,
+// Rows of A per load: all 128, or the next of 32 and 64 that holds every row there is.
+int a_box(int64_t rows, const Shape& s) { return s.pair || rows > 64 ? BM : rows > 32 ? 64 : 32; }
+
+// Cycles until the last SM is done: rounds of tiles, each the longest of
+//   its products: 4096 multiply-adds per cycle and SM;
+//   what it takes from L2: 10.2 TB/s measured with all SMs reading (256 x 256 pair tiles 459 ns per
+//   64-deep step, 256 x 128 ones 350 ns), 64 bytes per cycle and SM at most;
+//   the weights from HBM where no other row tile reads them too (about 4.2 TB/s in such tiles);
+//   its epilogue, which overlaps the next tile's products.
+double estimate(const Shape& s, int mode, int64_t e, int64_t rows, int64_t cols, int64_t k, const DeviceInfo& d) {
+  if (s.pair && (d.pairs == 0 || rows <= BM)) return 1e30;
+  const int64_t tm = s.pair ? 2 * BM : BM, tn = mode == 0 ? s.bn / 2 : s.bn;
+  const int64_t row_tiles = (rows + tm - 1) / tm, tiles = e * row_tiles * ((cols + tn - 1) / tn);
+  const int64_t units = s.pair ? d.pairs : d.sms;
+  const double rounds = static_cast<double>((tiles + units - 1) / units);
+  const double busy = static_cast<double>((tiles < units ? tiles : units) * (s.pair ? 2 : 1));
+  const double b_bytes = (s.pair ? s.bn / 2 : s.bn) * ROW_BYTES, a_bytes = a_box(rows, s) * ROW_BYTES;
+  double step = 2.0 * s.bn;
+  const double l2 = 5500.0 / busy < 64.0 ? 5500.0 / busy : 64.0;
+  if ((a_bytes + b_bytes) / l2 > step) step = (a_bytes + b_bytes) / l2;
+  if (row_tiles == 1 && b_bytes * busy / 2300.0 > step) step = b_bytes * busy / 2300.0;
+  const double epilogue = (mode < 2 ? 900.0 : 500.0) * ((tn + 63) / 64);
+  const double work = step * ((k + BK - 1) / BK);
+  return rounds * (work > epilogue ? work : epilogue) + epilogue + 1500.0;
+}
+
+Shape choose_shape(int mode, int64_t e, int64_t rows, int64_t cols, int64_t k, const DeviceInfo& d) {
+  Shape best = SHAPES[0];
+  double best_cycles = estimate(best, mode, e, rows, cols, k, d);
+  for (const Shape& s : SHAPES) {
+    const double c = estimate(s, mode, e, rows, cols, k, d);
+    if (c < best_cycles) {
+      best = s;
+      best_cycles = c;
+    }
+  }
+  return best;
+}
+
+int launch(int mode, const Shape& s, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh,
+           const CUtensorMap& ms, const CUtensorMap& md, GatedParams p, const DeviceInfo& info,
            cudaStream_t stream) {
-  const int tm = pair ? 2 * BM : BM, tn = MODE == 0 ? HALF : BN;
+  const int tm = s.pair ? 2 * BM : BM, tn = mode == 0 ? s.bn / 2 : s.bn;
   const long long tiles =
       static_cast<long long>(p.batch) * ((p.rows + tm - 1) / tm) * ((p.m + tn - 1) / tn);
   if (tiles > 0x7fffffff) return fail("gated mlp: too many tiles");
-  const long long most = pair ? info.pairs : info.sms;
+  p.a_box = a_box(p.rows, s);
+  p.stages = PIPE_BYTES / ((p.a_box + (s.pair ? s.bn / 2 : s.bn)) * ROW_BYTES);
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  const long long most = s.pair ? info.pairs : info.sms;
   const unsigned units = static_cast<unsigned>(tiles < most ? tiles : most);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -717,15 +847,13 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh, 
   attr.val.clusterDim.x = 2;
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3(pair ? 2 * units : units);
+  cfg.gridDim = dim3(s.pair ? 2 * units : units);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = pair ? 1 : 0;
-  const cudaError_t e =
-      pair ? cudaLaunchKernelEx(&cfg, gated_kernel<true, MODE>, ma, mb, mh, ms, md, p)
-           : cudaLaunchKernelEx(&cfg, gated_kernel<false, MODE>, ma, mb, mh, ms, md, p);
+  cfg.numAttrs = s.pair ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(mode, s), ma, mb, mh, ms, md, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
@@ -755,12 +883,6 @@ int check_sizes(const VmoeGatedArgs* a) {
     if (reinterpret_cast<uintptr_t>(q) & 15) return fail("gated mlp: operands must be 16-byte aligned");
   if (a->act != 0 && a->act != 1) return fail("gated mlp: unknown activation");
   return 0;
-}
-
-bool use_pairs(const VmoeGatedArgs* a, const DeviceInfo& info, int tn) {
-  // Pairs pay off once there is a 256-row tile for at least every other pair of SMs.
-  const long long tiles = a->e * ((a->rows + 2 * BM - 1) / (2 * BM)) * ((a->m + tn - 1) / tn);
-  return info.pairs > 0 && a->rows >= 2 * BM && tiles >= info.pairs / 2;
 }
 
 // The few-row kernel: rows of x in groups of 8.
@@ -862,6 +984,48 @@ void gemm_operands(VmoeGemmArgs* g, const void* a, int64_t lda, int64_t sa, int 
   g->split_k = 1;
 }
 
+// out (e, rows, n) = a (e, rows, k) b^T + bias + residual, b (e, n, k) or, with b_mn, (e, k, n): on this
+// file's tiles or on the plain GEMM, whichever is estimated to be done first. bias_f32: the plain GEMM's
+// form of a bf16 bias.
+int product(const void* a, const void* b, int b_mn, const void* bias, int bias_bf16, const float* bias_f32,
+            const void* residual, int64_t ldr, int64_t r_batch_stride, void* out, int64_t e, int64_t rows,
+            int64_t n, int64_t k, const DeviceInfo& info, cudaStream_t stream) {
+  const int mode = b_mn ? 3 : 2;
+  const Shape s = choose_shape(mode, e, rows, n, k, info);
+  if (s.bn == 256) {
+    VmoeGemmArgs g;
+    gemm_operands(&g, a, k, rows * k, 0, b, b_mn ? n : k, n * k, b_mn, rows, n, k, e);
+    g.C = out;
+    g.bias = bias_bf16 ? bias_f32 : static_cast<const float*>(bias);
+    g.bias_batch_stride = e > 1 ? n : 0;
+    g.residual = residual;
+    g.ldr = ldr;
+    g.r_batch_stride = e > 1 ? r_batch_stride : 0;
+    return vmoe_gemm_bf16(&g, stream);
+  }
+  CUtensorMap ma, mb, mh;
+  int rc;
+  if ((rc = make_bf16_map(&ma, a, k, rows, e, k, rows * k, a_box(rows, s), 64, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  const int b_rows = s.pair ? s.bn / 2 : s.bn;
+  if ((rc = b_mn ? make_bf16_map(&mb, b, n, k, e, n, n * k, BK, 64, CU_TENSOR_MAP_SWIZZLE_128B)
+                 : make_bf16_map(&mb, b, k, n, e, k, n * k, b_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_bf16_map(&mh, out, n, rows, e, n, rows * n, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
+  GatedParams p;
+  memset(&p, 0, sizeof(p));
+  p.bias = bias;
+  p.bias_bf16 = bias_bf16;
+  p.residual = static_cast<const __nv_bfloat16*>(residual);
+  p.ldr = ldr;
+  p.r_batch_stride = r_batch_stride;
+  p.rows = static_cast<int>(rows);
+  p.k = static_cast<int>(k);
+  p.m = static_cast<int>(n);
+  p.batch = static_cast<int>(e);
+  return launch(mode, s, ma, mb, mh, mh, mh, p, info, stream);
+}
+
 // Pieces that a weight gradient's contraction over `rows` is cut into: few output tiles leave SMs
 // idle in the last round, each piece costs writing and reading its fp32 result once.
 int gradient_pieces(int64_t e, int64_t n, int64_t k, int64_t rows) {
@@ -954,10 +1118,11 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   if (a->rows <= FEW_ROWS) return few_rows(a, info, stream);
   CUtensorMap ma, mb, mh, ms;
   memset(&ms, 0, sizeof(ms));
-  if ((rc = make_bf16_map(&ma, a->x, a->h, a->rows, a->e, a->h, a->rows * a->h, BM, 64,
+  const Shape shape = choose_shape(0, a->e, a->rows, a->m, a->h, info);
+  if ((rc = make_bf16_map(&ma, a->x, a->h, a->rows, a->e, a->h, a->rows * a->h, a_box(a->rows, shape), 64,
                           CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
-  if ((rc = make_bf16_map(&mb, a->w_in, a->h, a->m, 2 * a->e, a->h, a->m * a->h, HALF, 64,
+  if ((rc = make_bf16_map(&mb, a->w_in, a->h, a->m, 2 * a->e, a->h, a->m * a->h, shape.bn / 2, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
   if ((rc = make_bf16_map(&mh, a->hid, a->m, a->rows, a->e, a->m, a->rows * a->m, 32, 32,
@@ -968,8 +1133,7 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   memset(&p, 0, sizeof(p));
   p.bias = a->b_in;
   p.bias_bf16 = a->b_in_bf16;
-  const bool convert = a->b_out && a->b_out_bf16;
-  if (convert) {
+  if (a->b_out && a->b_out_bf16) {
     if (!a->scratch) return fail("gated mlp: scratch is missing");
     p.bias_out = static_cast<const __nv_bfloat16*>(a->b_out);
     p.bias_out_f32 = a->scratch;
@@ -981,17 +1145,9 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   p.batch = static_cast<int>(a->e);
   p.act = a->act;
   p.save = a->saved != nullptr;
-  if ((rc = launch<0>(ma, mb, mh, ms, ms, p, info, use_pairs(a, info, HALF), stream))) return rc;
-  VmoeGemmArgs g;
-  gemm_operands(&g, a->hid, a->m, a->rows * a->m, 0, a->w_out, a->m, a->o * a->m, 0, a->rows, a->o, a->m,
-                a->e);
-  g.C = a->y;
-  g.bias = convert ? a->scratch : static_cast<const float*>(a->b_out);
-  g.bias_batch_stride = a->e > 1 ? a->o : 0;
-  g.residual = a->residual;
-  g.ldr = a->ld_res;
-  g.r_batch_stride = a->e > 1 ? a->res_batch_stride : 0;
-  return vmoe_gemm_bf16(&g, stream);
+  if ((rc = launch(0, shape, ma, mb, mh, ms, ms, p, info, stream))) return rc;
+  return product(a->hid, a->w_out, 0, a->b_out, a->b_out_bf16, a->scratch, a->residual, a->ld_res,
+                 a->res_batch_stride, a->y, a->e, a->rows, a->o, a->m, info, stream);
 }
 
 extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
@@ -1018,7 +1174,8 @@ extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   }
   if (a->rows > 0 && inner) {
     CUtensorMap ma, mb, ms, md;
-    if ((rc = make_bf16_map(&ma, a->dy, a->o, a->rows, a->e, a->o, a->rows * a->o, BM, 64,
+    const Shape shape = choose_shape(1, a->e, a->rows, a->m, a->o, info);
+    if ((rc = make_bf16_map(&ma, a->dy, a->o, a->rows, a->e, a->o, a->rows * a->o, a_box(a->rows, shape), 64,
                             CU_TENSOR_MAP_SWIZZLE_128B)))
       return rc;
     if ((rc = make_bf16_map(&mb, a->w_out, a->m, a->o, a->e, a->m, a->m * a->o, BK, 64,
@@ -1033,7 +1190,7 @@ extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
     p.k = static_cast<int>(a->o);
     p.m = static_cast<int>(a->m);
     p.batch = static_cast<int>(a->e);
-    if ((rc = launch<1>(ma, mb, ms, ms, md, p, info, use_pairs(a, info, BN), stream))) return rc;
+    if ((rc = launch(1, shape, ma, mb, ms, ms, md, p, info, stream))) return rc;
   }
   if (a->db_in || a->db_out) {
     SumsPart u = {sums, a->db_in, static_cast<int>((a->rows + 31) / 32),
@@ -1046,13 +1203,10 @@ extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
                              256, 0, stream>>>(u, v);
     if ((rc = check_launch())) return rc;
   }
-  if (a->dx && a->rows > 0) {
-    VmoeGemmArgs g;
-    gemm_operands(&g, a->dgu, 2 * a->m, a->rows * 2 * a->m, 0, a->w_in, a->h, 2 * a->m * a->h, 1, a->rows,
-                  a->h, 2 * a->m, a->e);
-    g.C = a->dx;
-    if ((rc = vmoe_gemm_bf16(&g, stream))) return rc;
-  }
+  if (a->dx && a->rows > 0 &&
+      (rc = product(a->dgu, a->w_in, 1, nullptr, 0, nullptr, nullptr, 0, 0, a->dx, a->e, a->rows, a->h,
+                    2 * a->m, info, stream)))
+    return rc;
   if (a->dw_in && (rc = weight_gradient(a->dgu, a->x, a->e, a->rows, 2 * a->m, a->h, a->dw_in,
                                         a->dw_in_mode, pieces, stream)))
     return rc;
