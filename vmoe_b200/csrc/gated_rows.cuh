@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(GR_THREADS) gated_rows_kernel(const RowsParams
         gate += load_bias(p.bias, p.bias_bf16, 2ll * e * p.m + m);
         up += load_bias(p.bias, p.bias_bf16, (2ll * e + 1) * p.m + m);
       }
-      float a, slope;
-      gate_and_slope(gate, p.act, a, slope);
+      float a, slope, unused_a, unused_slope;
+      gate_and_slope(gate, gate, p.act, a, unused_a, slope, unused_slope);
       p.out[at] = __float2bfloat16(a * up);
       if (p.saved) {
         const long long sat = (static_cast<long long>(e) * p.rows + row) * 2 * p.m + m;

@@ -48,11 +48,15 @@ constexpr int MAX_STAGES = 10;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TILE_BYTES = 32 * 32 * 2;     // one staging tile: 32 rows of 64 bytes, 64B swizzle
-constexpr int EPI_TILES = 4;                // per epilogue warp
-constexpr int PIPE_BYTES = 160 * 1024;      // stages of A rows and B rows, as many as fit
-constexpr int SMEM_BYTES = PIPE_BYTES + EPI_WARPS * EPI_TILES * TILE_BYTES + 1024 + 320;
+constexpr int IN_BUFFERS = 3;               // backward: chunks of saved factors in flight or in use
+// Staging tiles per epilogue warp, and stages of A rows and B rows, as many as fit the rest.
+__host__ __device__ constexpr int epi_bytes(int mode) {
+  return EPI_WARPS * (mode == 1 ? 2 * IN_BUFFERS : 4) * TILE_BYTES;
+}
+__host__ __device__ constexpr int pipe_bytes(int mode) { return (224 * 1024) - epi_bytes(mode); }
+constexpr int SMEM_BYTES = 224 * 1024 + 1024 + 448;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
-static_assert((2 * MAX_STAGES + 4 + EPI_WARPS) * 8 + 8 <= 320, "room for the barriers");
+static_assert((2 * MAX_STAGES + 4 + EPI_WARPS * IN_BUFFERS) * 8 + 8 <= 448, "room for the barriers");
 
 // Tiled copies with four coordinates (column, factor, row, expert).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int c0,
@@ -73,24 +77,28 @@ __device__ __forceinline__ void tma_store_4d(const void* desc, uint32_t src, int
       : "memory");
 }
 
-// act(g) and act'(g) through one sigmoid: act = g sigma(w), act' = sigma (1 + g (1 - sigma) w').
-// GELU's tanh form is w = 2 sqrt(2/pi) (g + 0.044715 g^3), SiLU is w = g.
-__device__ __forceinline__ void gate_and_slope(float g, int act, float& a, float& slope) {
+// act(g) and act'(g) of two values through one sigmoid each: act = g s(w), act' = s (1 + g (1 - s) w').
+// GELU's tanh form is w = 2 sqrt(2/pi) (g + 0.044715 g^3), SiLU is w = g. (ex2 and a reciprocal, 2^-22:
+// tanh.approx would save one of the two, but its 2^-11 is several bf16 steps of act and act' where they
+// fall off on the negative side.)
+__device__ __forceinline__ void gate_and_slope(float g0, float g1, int act, float& a0, float& a1, float& s0,
+                                               float& s1) {
   constexpr float K0 = 1.5957691216057308f, K1 = K0 * 0.044715f, L = 1.4426950408889634f;
-  float w, dw;
-  if (act == 0) {
-    const float g2 = g * g;
-    w = g * fmaf(g2, K1, K0);
-    dw = fmaf(g2, 3.0f * K1, K0);
-  } else {
-    w = g;
-    dw = 1.0f;
-  }
-  float e, sg;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-L * w));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.0f + e));
-  a = g * sg;
-  slope = sg * fmaf(g * (1.0f - sg), dw, 1.0f);
+  const float k0 = act == 0 ? K0 : 1.0f, k1 = act == 0 ? K1 : 0.0f;
+  const f32x2 g = f2_pack(g0, g1), one = f2_pack(1.0f, 1.0f);
+  const f32x2 g2 = f2_mul(g, g);
+  float u0, u1, r0, r1;
+  f2_unpack(f2_mul(g, f2_fma(g2, f2_pack(-L * k1, -L * k1), f2_pack(-L * k0, -L * k0))), u0, u1);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u1));
+  f2_unpack(f2_add(f2_pack(u0, u1), one), r0, r1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r1));
+  const f32x2 s = f2_pack(r0, r1);
+  const f32x2 rest = f2_fma(s, f2_pack(-1.0f, -1.0f), one);
+  const f32x2 dw = f2_fma(g2, f2_pack(3.0f * k1, 3.0f * k1), f2_pack(k0, k0));
+  f2_unpack(f2_mul(g, s), a0, a1);
+  f2_unpack(f2_mul(s, f2_fma(f2_mul(g, rest), dw, one)), s0, s1);
 }
 
 struct GatedParams {
@@ -140,15 +148,15 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   const int a_stage = max(p.a_box, 8) * ROW_BYTES;
   uint8_t* sA = smem;
   uint8_t* sB = smem + nstage * a_stage;
-  uint8_t* sEpi = smem + PIPE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + EPI_WARPS * EPI_TILES * TILE_BYTES);
-  // full[stages], empty[stages], accumulator full[2], accumulator empty[2], epilogue input[8]
+  uint8_t* sEpi = smem + pipe_bytes(MODE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + epi_bytes(MODE));
+  // full[stages], empty[stages], accumulator full[2], accumulator empty[2], epilogue input[8][3]
   const uint32_t bar_full = smem_u32(bars);
   const uint32_t bar_empty = smem_u32(bars + nstage);
   const uint32_t bar_tfull = smem_u32(bars + 2 * nstage);
   const uint32_t bar_tempty = smem_u32(bars + 2 * nstage + 2);
   const uint32_t bar_in = smem_u32(bars + 2 * nstage + 4);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * nstage + 4 + EPI_WARPS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * nstage + 4 + EPI_WARPS * IN_BUFFERS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int cta = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -166,7 +174,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       mbar_init(bar_tfull + 8 * s, 1);
       mbar_init(bar_tempty + 8 * s, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
-    for (int s = 0; s < EPI_WARPS; ++s) mbar_init(bar_in + 8 * s, 1);
+    for (int s = 0; s < EPI_WARPS * IN_BUFFERS; ++s) mbar_init(bar_in + 8 * s, 1);
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
@@ -314,13 +322,12 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     const int ew = warp - 2;
     const int quad = warp & 3;   // TMEM lanes this warp may read
     const int half = ew >> 2;
-    uint8_t* tiles = sEpi + ew * EPI_TILES * TILE_BYTES;
+    uint8_t* tiles = sEpi + ew * (epi_bytes(MODE) / EPI_WARPS);
     const uint32_t st_row = static_cast<uint32_t>(lane) * 64u;
     const uint32_t st_xor = (static_cast<uint32_t>(lane) >> 1) & 3u;
     constexpr int CHUNKS = TN / 32;  // 32-column chunks of a tile, shared by two warps per quadrant
-    const uint32_t in_bar = bar_in + 8 * ew;
+    const uint32_t in_bar = bar_in + 8 * IN_BUFFERS * ew;
     const uint32_t tempty_base = PAIR ? mapa_shared(bar_tempty, 0) : bar_tempty;
-    uint32_t in_phase = 0;
     int local = 0;
     bool ok = true;
     if (MODE == 0 && p.bias_out)  // the GEMM behind this kernel takes fp32 biases
@@ -334,6 +341,34 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         *reinterpret_cast<uint4*>(tile + st_row + ((static_cast<uint32_t>(i) ^ st_xor) << 4)) =
             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     };
+    // Backward: this warp's chunks over all its tiles, in order. The saved factors of a chunk arrive in one
+    // of IN_BUFFERS pairs of tiles, where dg and du take their place and leave. Loads run two chunks
+    // ahead (a load takes longer than a chunk's arithmetic), into the next tiles too.
+    int ahead_tile = cta, ahead_c = half - 2, ahead = 0, done = 0;
+    auto fetch_next = [&]() {
+      while (ahead_tile < num_tiles) {
+        int b, mt, nt;
+        decode(ahead_tile, b, mt, nt);
+        ahead_c += 2;
+        const int col = nt * TN + ahead_c * 32;
+        if (ahead_c < CHUNKS && col < p.m) {
+          if (lane == 0) {
+            const int buf = ahead % IN_BUFFERS;
+            const uint32_t dst = smem_u32(tiles + buf * 2 * TILE_BYTES);
+            const int row = mt * TM + static_cast<int>(rank) * BM + quad * 32;
+            mbar_expect_tx(in_bar + 8 * buf, 2 * TILE_BYTES);
+            tma_load_4d(dst, &map_s, in_bar + 8 * buf, col, 0, row, b);
+            tma_load_4d(dst + TILE_BYTES, &map_s, in_bar + 8 * buf, col, 1, row, b);
+          }
+          ++ahead;
+          return;
+        }
+        ahead_tile += ncta;
+        ahead_c = half - 2;
+      }
+    };
+    if (MODE == 1)
+      for (int i = 0; i < IN_BUFFERS - 1; ++i) fetch_next();
     for (int tile = cta; tile < num_tiles && ok; tile += ncta, ++local) {
       int b, mt, nt;
       decode(tile, b, mt, nt);
@@ -341,15 +376,6 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       const uint32_t use = static_cast<uint32_t>(local >> 1);
       const int row0 = mt * TM + static_cast<int>(rank) * BM + quad * 32;
       const int n0 = nt * TN;
-      // Backward: the saved factors of a chunk (tiles 2 and 3), fetched ahead.
-      auto fetch = [&](int col0) {
-        if (lane == 0) {
-          mbar_expect_tx(in_bar, 2 * TILE_BYTES);
-          tma_load_4d(smem_u32(tiles + 2 * TILE_BYTES), &map_s, in_bar, col0, 0, row0, b);
-          tma_load_4d(smem_u32(tiles + 3 * TILE_BYTES), &map_s, in_bar, col0, 1, row0, b);
-        }
-      };
-      if (MODE == 1 && n0 + half * 32 < p.m) fetch(n0 + half * 32);
       const bool got = mbar_wait(bar_tfull + 8 * slot, use & 1, abort_flag, nullptr, 0);
       if (!__all_sync(0xffffffffu, got)) {
         ok = false;
@@ -416,8 +442,7 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           for (int i = 0; i < 16; ++i) {
             float a0, a1, s0, s1;
             const float u0 = __uint_as_float(ru[2 * i]), u1 = __uint_as_float(ru[2 * i + 1]);
-            gate_and_slope(__uint_as_float(rg[2 * i]), p.act, a0, s0);
-            gate_and_slope(__uint_as_float(rg[2 * i + 1]), p.act, a1, s1);
+            gate_and_slope(__uint_as_float(rg[2 * i]), __uint_as_float(rg[2 * i + 1]), p.act, a0, a1, s0, s1);
             wh[i] = pack_bf16x2(a0 * u0, a1 * u1);
             wa[i] = pack_bf16x2(a0, a1);
             ws[i] = pack_bf16x2(s0 * u0, s1 * u1);
@@ -499,8 +524,10 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         } else {
           uint32_t r[32];
           tmem_ld_32x32(acc, r);
-          const bool in = mbar_wait(in_bar, in_phase, abort_flag, nullptr, 0);
-          in_phase ^= 1;
+          uint8_t* factors = tiles + (done % IN_BUFFERS) * 2 * TILE_BYTES;
+          const bool in = mbar_wait(in_bar + 8 * (done % IN_BUFFERS), (done / IN_BUFFERS) & 1, abort_flag,
+                                    nullptr, 0);
+          ++done;
           if (!__all_sync(0xffffffffu, in)) {
             ok = false;
             break;
@@ -509,12 +536,10 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t off = st_row + ((static_cast<uint32_t>(i) ^ st_xor) << 4);
-            qs[i] = *reinterpret_cast<const uint4*>(tiles + 2 * TILE_BYTES + off);
-            qa[i] = *reinterpret_cast<const uint4*>(tiles + 3 * TILE_BYTES + off);
+            qs[i] = *reinterpret_cast<const uint4*>(factors + off);
+            qa[i] = *reinterpret_cast<const uint4*>(factors + TILE_BYTES + off);
           }
           tmem_ld_wait();
-          __syncwarp();
-          if (c + 2 < CHUNKS && col0 + 64 < p.m) fetch(col0 + 64);
           uint32_t wg[16], wu[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -526,15 +551,18 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             wg[i] = pack_bf16x2(d0 * fs.x, d1 * fs.y);
             wu[i] = pack_bf16x2(d0 * fa.x, d1 * fa.y);
           }
+          // The chunk before this one has left its buffer (and every lane has read its column sums):
+          // that buffer takes the chunk after the next.
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          stage_row(tiles, wg);
-          stage_row(tiles + TILE_BYTES, wu);
+          fetch_next();
+          stage_row(factors, wg);  // a lane overwrites the row that it has read
+          stage_row(factors + TILE_BYTES, wu);
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            tma_store_4d(&map_d, smem_u32(tiles), col0, 0, row0, b);
-            tma_store_4d(&map_d, smem_u32(tiles + TILE_BYTES), col0, 1, row0, b);
+            tma_store_4d(&map_d, smem_u32(factors), col0, 0, row0, b);
+            tma_store_4d(&map_d, smem_u32(factors + TILE_BYTES), col0, 1, row0, b);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
           if (p.sums && row0 < p.rows) {
@@ -542,21 +570,21 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             // of two columns each (rows past the end hold zeros). Written, not added: a second
             // kernel joins the row blocks in a fixed order.
             const long long blocks = (p.rows + 31) / 32;
-            const uint32_t pair = lane & 15, odd = lane >> 4;
+            const uint32_t two = lane & 15, odd = lane >> 4;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const uint32_t rr = 2 * i + odd;
-                const uint32_t off = rr * 64u + (((pair >> 2) ^ ((rr >> 1) & 3u)) << 4) + (pair & 3) * 4u;
-                const float2 f = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(tiles + w * TILE_BYTES + off));
+                const uint32_t off = rr * 64u + (((two >> 2) ^ ((rr >> 1) & 3u)) << 4) + (two & 3) * 4u;
+                const float2 f = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(factors + w * TILE_BYTES + off));
                 s0 += f.x;
                 s1 += f.y;
               }
               s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
               s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
-              const int col = col0 + 2 * static_cast<int>(pair);
+              const int col = col0 + 2 * static_cast<int>(two);
               if (odd == 0 && col < p.m)
                 *reinterpret_cast<float2*>(p.sums + ((b * blocks + row0 / 32) * 2 + w) * p.m + col) =
                     make_float2(s0, s1);
@@ -835,7 +863,7 @@ int launch(int mode, const Shape& s, const CUtensorMap& ma, const CUtensorMap& m
       static_cast<long long>(p.batch) * ((p.rows + tm - 1) / tm) * ((p.m + tn - 1) / tn);
   if (tiles > 0x7fffffff) return fail("gated mlp: too many tiles");
   p.a_box = a_box(p.rows, s);
-  p.stages = PIPE_BYTES / ((p.a_box + (s.pair ? s.bn / 2 : s.bn)) * ROW_BYTES);
+  p.stages = pipe_bytes(mode) / ((p.a_box + (s.pair ? s.bn / 2 : s.bn)) * ROW_BYTES);
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const long long most = s.pair ? info.pairs : info.sms;
   const unsigned units = static_cast<unsigned>(tiles < most ? tiles : most);
