@@ -208,20 +208,25 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t full_base = PAIR ? mapa_shared(bar_full, 0) : bar_full;
-      for (int tile = cta; tile < num_tiles && ok; tile += ncta) {
-        int b, mt, nt;
-        decode(tile, b, mt, nt);
-        const int m0 = mt * TM + static_cast<int>(rank) * BM;
-        for (int kt = 0; kt < k_tiles; ++kt) {
-          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, nullptr, 0)) {
-            ok = false;
-            break;
-          }
+    // The whole warp walks through the steps and one elected thread issues: operands of the copies (and
+    // of the products below) then are uniform across the warp. One thread alone in a branch of its own
+    // took 290 ns per 64-deep step whatever the tile.
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full_base = PAIR ? mapa_shared(bar_full, 0) : bar_full;
+    for (int tile = cta; tile < num_tiles && ok; tile += ncta) {
+      int b, mt, nt;
+      decode(tile, b, mt, nt);
+      const int m0 = mt * TM + static_cast<int>(rank) * BM;
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        const bool got = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, nullptr, 0);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        if (leader) {
           const uint32_t full = full_base + 8 * stage;
           if (!PAIR) {
             mbar_expect_tx(full, a_stage + BSTAGE);
@@ -255,20 +260,22 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
               for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * CHUNK_BYTES, &map_b, n0 + 64 * j, k0, b);
             }
           }
-          if (++stage == nstage) {
-            stage = 0;
-            phase ^= 1;
-          }
+        }
+        __syncwarp();
+        if (++stage == nstage) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (!ok) {  // copies in flight get a bounded chance to land before the CTA exits
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000) __nanosleep(256);
-      }
+    }
+    if (!ok) {  // copies in flight get a bounded chance to land before the CTA exits
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000) __nanosleep(256);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool leader = elect_one();
       const uint32_t idesc = umma_idesc_bf16(TM, BN, 0, B_MN ? 1 : 0);
       const uint32_t b_lbo = B_MN ? CHUNK_BYTES : 16, b_step = B_MN ? 2048 : 32;
       int stage = 0;
@@ -278,42 +285,48 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       for (int tile = cta; tile < num_tiles && ok; tile += ncta, ++local) {
         const int slot = local & 1;
         const uint32_t use = static_cast<uint32_t>(local >> 1);
-        if (!mbar_wait(bar_tempty + 8 * slot, (use & 1) ^ 1, abort_flag, nullptr, 0)) break;
+        bool got = mbar_wait(bar_tempty + 8 * slot, (use & 1) ^ 1, abort_flag, nullptr, 0);
+        if (!__all_sync(0xffffffffu, got)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + slot * BN;
         for (int kt = 0; kt < k_tiles; ++kt) {
-          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, nullptr, 0)) {
+          got = mbar_wait(bar_full + 8 * stage, phase, abort_flag, nullptr, 0);
+          if (!__all_sync(0xffffffffu, got)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + stage * a_stage);
-          const uint32_t b_addr = smem_u32(sB + stage * BSTAGE);
+          if (leader) {
+            const uint32_t a_addr = smem_u32(sA + stage * a_stage);
+            const uint32_t b_addr = smem_u32(sB + stage * BSTAGE);
 #pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k) {
-            const uint64_t adesc = umma_smem_desc(a_addr + k * 32, 16, 1024);
-            const uint64_t bdesc = umma_smem_desc(b_addr + k * b_step, b_lbo, 1024);
+            for (int k = 0; k < BK / UMMA_K; ++k) {
+              const uint64_t adesc = umma_smem_desc(a_addr + k * 32, 16, 1024);
+              const uint64_t bdesc = umma_smem_desc(b_addr + k * b_step, b_lbo, 1024);
+              if (PAIR) {
+                umma_bf16_pair(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+              } else {
+                umma_bf16(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+              }
+            }
             if (PAIR) {
-              umma_bf16_pair(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+              umma_commit_pair(bar_empty + 8 * stage, 3);
             } else {
-              umma_bf16(d_tmem, adesc, bdesc, idesc, (kt > 0 || k > 0) ? 1u : 0u);
+              umma_commit(bar_empty + 8 * stage);
+            }
+            if (kt == k_tiles - 1) {
+              if (PAIR) {
+                umma_commit_pair(bar_tfull + 8 * slot, 3);
+              } else {
+                umma_commit(bar_tfull + 8 * slot);
+              }
             }
           }
-          if (PAIR) {
-            umma_commit_pair(bar_empty + 8 * stage, 3);
-          } else {
-            umma_commit(bar_empty + 8 * stage);
-          }
+          __syncwarp();
           if (++stage == nstage) {
             stage = 0;
             phase ^= 1;
           }
-        }
-        if (!ok) break;
-        if (PAIR) {
-          umma_commit_pair(bar_tfull + 8 * slot, 3);
-        } else {
-          umma_commit(bar_tfull + 8 * slot);
         }
       }
     }
@@ -819,37 +832,31 @@ int device_info(DeviceInfo* out) {
 // Rows of A per load: all 128, or the next of 32 and 64 that holds every row there is.
 int a_box(int64_t rows, const Shape& s) { return s.pair || rows > 64 ? BM : rows > 32 ? 64 : 32; }
 
-// Cycles until the last SM is done: rounds of tiles, each the longest of
-//   its products: 4096 multiply-adds per cycle and SM;
-//   what it takes from L2: 10.2 TB/s measured with all SMs reading (256 x 256 pair tiles 459 ns per
-//   64-deep step, 256 x 128 ones 350 ns), 64 bytes per cycle and SM at most;
-//   the weights from HBM where no other row tile reads them too (about 4.2 TB/s in such tiles);
-//   its epilogue, which overlaps the next tile's products.
+// Nanoseconds until the last SM is done: rounds of tiles, each the longer of its 64-deep steps and its
+// epilogue, which overlaps the next tile's steps. Measured over ten sizes from 16 x 64 rows of 512 x 1024 to
+// 2600 rows of 1024 x 2736: a step takes 400 ns on 256 x 256 pair tiles, 265 on 256 x 128 ones, 300 and
+// 255 on single 128 x 128 and 128 x 64 tiles (each product needs shared memory for its operands twice, for
+// the copy in and for the tensor core; small tiles reuse them less); an epilogue 2.5 us per 64
+// hidden units forward, 1.4 us backward, 1.2 us per 64 plain columns.
 double estimate(const Shape& s, int mode, int64_t e, int64_t rows, int64_t cols, int64_t k, const DeviceInfo& d) {
   if (s.pair && (d.pairs == 0 || rows <= BM)) return 1e30;
   const int64_t tm = s.pair ? 2 * BM : BM, tn = mode == 0 ? s.bn / 2 : s.bn;
-  const int64_t row_tiles = (rows + tm - 1) / tm, tiles = e * row_tiles * ((cols + tn - 1) / tn);
-  const int64_t units = s.pair ? d.pairs : d.sms;
+  const int64_t tiles = e * ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn), units = s.pair ? d.pairs : d.sms;
   const double rounds = static_cast<double>((tiles + units - 1) / units);
-  const double busy = static_cast<double>((tiles < units ? tiles : units) * (s.pair ? 2 : 1));
-  const double b_bytes = (s.pair ? s.bn / 2 : s.bn) * ROW_BYTES, a_bytes = a_box(rows, s) * ROW_BYTES;
-  double step = 2.0 * s.bn;
-  const double l2 = 5500.0 / busy < 64.0 ? 5500.0 / busy : 64.0;
-  if ((a_bytes + b_bytes) / l2 > step) step = (a_bytes + b_bytes) / l2;
-  if (row_tiles == 1 && b_bytes * busy / 2300.0 > step) step = b_bytes * busy / 2300.0;
-  const double epilogue = (mode < 2 ? 900.0 : 500.0) * ((tn + 63) / 64);
+  const double step = s.pair ? (s.bn == 256 ? 400.0 : 265.0) : (s.bn == 128 ? 300.0 : 255.0);
+  const double epilogue = (mode == 0 ? 2500.0 : mode == 1 ? 1400.0 : 1200.0) * tn / 64;
   const double work = step * ((k + BK - 1) / BK);
-  return rounds * (work > epilogue ? work : epilogue) + epilogue + 1500.0;
+  return rounds * (work > epilogue ? work : epilogue) + epilogue + (s.pair ? 1000.0 : 0.0);
 }
 
 Shape choose_shape(int mode, int64_t e, int64_t rows, int64_t cols, int64_t k, const DeviceInfo& d) {
   Shape best = SHAPES[0];
-  double best_cycles = estimate(best, mode, e, rows, cols, k, d);
+  double best_ns = estimate(best, mode, e, rows, cols, k, d);
   for (const Shape& s : SHAPES) {
-    const double c = estimate(s, mode, e, rows, cols, k, d);
-    if (c < best_cycles) {
+    const double ns = estimate(s, mode, e, rows, cols, k, d);
+    if (ns < best_ns) {
       best = s;
-      best_cycles = c;
+      best_ns = ns;
     }
   }
   return best;
@@ -1024,6 +1031,7 @@ int product(const void* a, const void* b, int b_mn, const void* bias, int bias_b
     VmoeGemmArgs g;
     gemm_operands(&g, a, k, rows * k, 0, b, b_mn ? n : k, n * k, b_mn, rows, n, k, e);
     g.C = out;
+    g.cta_pair = 2;  // the tiles of the estimate
     g.bias = bias_bf16 ? bias_f32 : static_cast<const float*>(bias);
     g.bias_batch_stride = e > 1 ? n : 0;
     g.residual = residual;
