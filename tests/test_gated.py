@@ -155,6 +155,8 @@ SHAPES = [
     (5, 100, 64, 72, None, False, True),
     (1, 1285, 256, 680, 1280, True, True),
     (1, 400, 520, 2048, None, True, False),
+    (32, 3, 136, 344, None, True, True),
+    (20, 11, 328, 264, 400, False, False),
 ]
 
 

@@ -3,9 +3,11 @@
 //
 // With R <= 16 rows the work is reading the weights (2 M K and O M elements), a few microseconds of
 // HBM time, so what counts is how soon all of them are in flight. A CTA takes 16 hidden units (their
-// gate and their up row) or 16 outputs; its 8 warps, and the 1, 2, 4 or 8 CTAs of a cluster when
-// there are few units, share the contraction in chunks of 32 elements, and a warp loads all its
-// first chunks before it needs one. m16n8k16 products take 16 weight rows as A and 8 rows of x as
+// gate and their up row) or 16 outputs; its warps, and the 1, 2, 4 or 8 CTAs of a cluster when
+// there are few units, share the contraction in units of 64 elements (a 128-byte line of every row;
+// units of 32 took 12 % longer over 32 experts of 512 x 1024), and a warp has two units' loads in
+// flight. CTAs have 8 warps, or 4 when there are two CTAs for every SM anyway (32 experts x 4 rows
+// 512 -> 1024: 21 us against 28; 1 row 768 -> 2048: 9.7 us against 8.6). m16n8k16 products take 16 weight rows as A and 8 rows of x as
 // B; the contraction's order is free, so a thread's fragments of two products are 16 consecutive
 // bytes of a weight row and of a row of x, and neither needs shared memory. Partial sums meet in
 // shared memory, then over the cluster, in a fixed order. The tile kernel's 128-row tiles, TMA
@@ -20,10 +22,8 @@
 namespace vmoe {
 namespace {
 
-constexpr int GR_THREADS = 256;
-constexpr int GR_WARPS = GR_THREADS / 32;
 constexpr int GR_MAX_SPLIT = 8;
-constexpr int GR_AHEAD = 4;  // chunks a warp loads before it multiplies the first one
+constexpr int GR_AHEAD = 4;  // chunks of 32 elements a warp loads before it multiplies the first one
 
 struct RowsParams {
   const __nv_bfloat16* x;  // (E, rows, k)
@@ -59,8 +59,9 @@ __device__ __forceinline__ uint4 ld_stream(const __nv_bfloat16* p) {  // read on
 }
 
 // G weight groups of 16 rows: 2 (gate and up, gated = true) or 1; NT groups of 8 rows of x.
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(GR_THREADS) gated_rows_kernel(const RowsParams p) {
+template <int NT, bool GATED, int GR_THREADS>
+__global__ void __launch_bounds__(GR_THREADS, 512 / GR_THREADS) gated_rows_kernel(const RowsParams p) {
+  constexpr int GR_WARPS = GR_THREADS / 32;
   constexpr int G = GATED ? 2 : 1;
   constexpr int COLS = NT * 8;
   __shared__ float part[GR_WARPS][G][16][COLS + 1];
@@ -99,11 +100,11 @@ __global__ void __launch_bounds__(GR_THREADS) gated_rows_kernel(const RowsParams
 
   const uint4 zero = make_uint4(0, 0, 0, 0);
   bool waited = !p.after;
-  for (int c0 = first; c0 < chunks; c0 += GR_AHEAD * stride) {
-    uint4 wq[GR_AHEAD][G][2];
+  for (int c0 = first; c0 * 2 < chunks; c0 += GR_AHEAD / 2 * stride) {
+    uint4 wq[GR_AHEAD][G][2], xq[GR_AHEAD][NT];
 #pragma unroll
     for (int u = 0; u < GR_AHEAD; ++u) {
-      const int k0 = (c0 + u * stride) * 32 + t * 8;
+      const int k0 = (c0 + (u >> 1) * stride) * 64 + (u & 1) * 32 + t * 8;
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -116,18 +117,20 @@ __global__ void __launch_bounds__(GR_THREADS) gated_rows_kernel(const RowsParams
     }
 #pragma unroll
     for (int u = 0; u < GR_AHEAD; ++u) {
-      const int k0 = (c0 + u * stride) * 32 + t * 8;
-      uint4 xq[NT];
+      const int k0 = (c0 + (u >> 1) * stride) * 64 + (u & 1) * 32 + t * 8;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        xq[j] = k0 < p.k ? *reinterpret_cast<const uint4*>(xrow[j] + k0) : zero;
+        xq[u][j] = k0 < p.k ? *reinterpret_cast<const uint4*>(xrow[j] + k0) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < GR_AHEAD; ++u) {
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const uint4 a = wq[u][i][0], b = wq[u][i][1];
-          mma_16x8x16(acc[i][j], a.x, b.x, a.y, b.y, xq[j].x, xq[j].y);
-          mma_16x8x16(acc[i][j], a.z, b.z, a.w, b.w, xq[j].z, xq[j].w);
+          mma_16x8x16(acc[i][j], a.x, b.x, a.y, b.y, xq[u][j].x, xq[u][j].y);
+          mma_16x8x16(acc[i][j], a.z, b.z, a.w, b.w, xq[u][j].z, xq[u][j].w);
         }
     }
   }

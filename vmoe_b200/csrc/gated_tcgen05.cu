@@ -926,9 +926,11 @@ constexpr int FEW_ROWS = 16;
 template <int NT, bool GATED>
 int launch_rows(RowsParams p, int e, int sms, cudaStream_t stream) {
   const int tiles = (p.m + 15) / 16, chunks = (p.k + 31) / 32;
+  const int threads = tiles * e >= 2 * sms ? 128 : 256;
   // Share the contraction over a cluster until every SM has a CTA, while each warp keeps a chunk.
   p.split = 1;
-  while (p.split < GR_MAX_SPLIT && tiles * e * p.split < sms && chunks >= 2 * p.split * GR_WARPS) p.split *= 2;
+  while (p.split < GR_MAX_SPLIT && tiles * e * p.split < sms && chunks >= 2 * p.split * (threads / 32))
+    p.split *= 2;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cudaLaunchAttribute attr[2];
@@ -947,11 +949,12 @@ int launch_rows(RowsParams p, int e, int sms, cudaStream_t stream) {
     ++n;
   }
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split), static_cast<unsigned>(e));
-  cfg.blockDim = dim3(GR_THREADS);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, gated_rows_kernel<NT, GATED>, p);
+  const cudaError_t err = threads == 128 ? cudaLaunchKernelEx(&cfg, gated_rows_kernel<NT, GATED, 128>, p)
+                                         : cudaLaunchKernelEx(&cfg, gated_rows_kernel<NT, GATED, 256>, p);
   if (err != cudaSuccess) {
     cudaGetLastError();
     set_error("%s (code %d)", cudaGetErrorString(err), static_cast<int>(err));
