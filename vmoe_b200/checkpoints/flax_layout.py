@@ -5,7 +5,8 @@ Layouts (Flax side, as pinned by the reference's tests, ``vmoe/nn/vit_moe_test.p
 ``Dense/kernel (in, out)``; attention ``query|key|value/kernel (hidden, heads, head_dim)``,
 ``bias (heads, head_dim)``, ``out/kernel (heads, head_dim, hidden)``; patch embedding
 ``embedding/kernel (ph, pw, C, hidden)``; MLP ``Dense_0/kernel (hidden, mlp)``,
-``Dense_1/kernel (mlp, hidden)``; expert MLPs the same with a leading expert axis;
+``Dense_1/kernel (mlp, hidden)``; expert MLPs the same with a leading expert axis; gated MLPs
+``Dense_gate|Dense_up/kernel (hidden, mlp)``, ``Dense_out/kernel (mlp, hidden)``;
 ``Router/dense/kernel (hidden, experts)``. The PyTorch side stores GEMM weights as
 ``[out, in]`` (K-major for the tensor cores), fuses Q/K/V into one ``[3*hidden, hidden]``
 weight and gives dense MLPs a leading axis of 1.
@@ -48,6 +49,14 @@ def _entries(model: torch.nn.Module):
         kind = ("mlp_w" if pn.startswith("w") else "mlp_b") + ("_dense" if dense else "")
         yield join(fn), p, kind, None
         claimed.add(id(p))
+    elif isinstance(mod, (vit_moe.GatedMlpBlock, vit_moe.GatedExpertMlp)):
+      tail = "_dense" if isinstance(mod, vit_moe.GatedMlpBlock) else ""
+      for i, name in enumerate(("Dense_gate", "Dense_up")):
+        yield join(name, "kernel"), mod.w_in, "gated_w" + tail, i
+        yield join(name, "bias"), mod.b_in, "gated_b" + tail, i
+      yield join("Dense_out", "kernel"), mod.w_out, "mlp_w" + tail, None
+      yield join("Dense_out", "bias"), mod.b_out, "mlp_b" + tail, None
+      claimed.update(id(p) for p in (mod.w_in, mod.b_in, mod.w_out, mod.b_out))
     elif isinstance(mod, vit_moe.Dense):
       if id(mod.weight) in claimed:
         continue
@@ -107,6 +116,14 @@ def _to_flax_array(p: torch.Tensor, kind: str, extra) -> np.ndarray:
     out = t[0].t()
   elif kind == "mlp_b_dense":
     out = t[0]
+  elif kind == "gated_w":
+    out = t[:, extra].transpose(1, 2)
+  elif kind == "gated_b":
+    out = t[:, extra]
+  elif kind == "gated_w_dense":
+    out = t[0, extra].t()
+  elif kind == "gated_b_dense":
+    out = t[0, extra]
   else:
     raise ValueError(kind)
   out = out.contiguous()
@@ -134,11 +151,13 @@ def _from_flax_array(value: np.ndarray, p: torch.Tensor, kind: str, extra) -> to
     return v.reshape(-1, v.shape[-1]).t()
   if kind == "member_gating_w":
     return v.permute(1, 2, 0)
-  if kind == "mlp_w":
+  if kind in ("mlp_w", "gated_w"):
     return v.transpose(1, 2)
-  if kind == "mlp_w_dense":
+  if kind == "gated_b":
+    return v
+  if kind in ("mlp_w_dense", "gated_w_dense"):
     return v.t().unsqueeze(0)
-  if kind == "mlp_b_dense":
+  if kind in ("mlp_b_dense", "gated_b_dense"):
     return v.unsqueeze(0)
   raise ValueError(kind)
 
@@ -188,6 +207,8 @@ def from_flax(model: torch.nn.Module, params: Mapping[str, Any], mesh=None,
       i = extra[0]
       hid = p.shape[0] // 3
       p.data[i * hid:(i + 1) * hid].copy_(t.reshape(p.data[i * hid:(i + 1) * hid].shape))
+    elif kind.startswith("gated_"):
+      p.data[:, extra].copy_(t.reshape(p.data[:, extra].shape))
     else:
       p.data.copy_(t.reshape(p.shape))
   if strict and missing:

@@ -3,8 +3,9 @@ paths (slash separated). The paths are what regex options (weight decay, freezin
 scale, partitioning, tree summaries, initialization rules) are matched against, and the keys
 of V-MoE checkpoints.
 
-A fused tensor that corresponds to several Flax leaves (the QKV projection) reports the path
-of its first leaf (``.../query/...``).
+A fused tensor that corresponds to several Flax leaves (the QKV projection, the two input
+projections of a gated MLP) reports the path of its first leaf (``.../query/...``,
+``.../Dense_gate/...``).
 """
 from __future__ import annotations
 
@@ -12,6 +13,9 @@ _LEAF = {
     "weight": "kernel",
     "w1": "Dense_0/kernel", "b1": "Dense_0/bias",
     "w2": "Dense_1/kernel", "b2": "Dense_1/bias",
+    # Gated MLPs (no counterpart in the reference): one tensor for gate and up projection.
+    "w_in": "Dense_gate/kernel", "b_in": "Dense_gate/bias",
+    "w_out": "Dense_out/kernel", "b_out": "Dense_out/bias",
 }
 
 

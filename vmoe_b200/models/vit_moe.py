@@ -157,6 +157,86 @@ class ExpertMlp(nn.Module):
     return ops.expert_mlp(x, self.w1, self.b1, self.w2, self.b2)
 
 
+def _gated_parameters(num_experts: int, hidden_size: int, mlp_dim: int, out_dim: int):
+  """``w_in (E, 2, M, H)`` (gate's projection first), ``b_in``, ``w_out (E, O, M)``, ``b_out``, initialised
+  like the two layers of the plain MLP."""
+  w_in = torch.empty(num_experts, 2, mlp_dim, hidden_size)
+  w_out = torch.empty(num_experts, out_dim, mlp_dim)
+  b_in, b_out = torch.empty(num_experts, 2, mlp_dim), torch.empty(num_experts, out_dim)
+  xavier_uniform_(w_in, hidden_size, mlp_dim)
+  xavier_uniform_(w_out, mlp_dim, out_dim)
+  nn.init.normal_(b_in, std=1e-6)
+  nn.init.normal_(b_out, std=1e-6)
+  return w_in, b_in, w_out, b_out
+
+
+def _gated_with_dropout(x, w_in, b_in, w_out, b_out, gate: str, rate: float):
+  """The gated MLP with dropout on the hidden units and on the output, in PyTorch ops."""
+  dt = x.dtype
+  g, u = (torch.baddbmm(b_in[:, i].to(dt).unsqueeze(1), x, w_in[:, i].to(dt).transpose(1, 2))
+          for i in (0, 1))
+  h = (F.silu(g) if gate == "silu" else F.gelu(g, approximate="tanh")) * u
+  y = torch.baddbmm(b_out.to(dt).unsqueeze(1), F.dropout(h, rate, True),
+                    w_out.to(dt).transpose(1, 2))
+  return F.dropout(y, rate, True)
+
+
+class GatedMlpBlock(nn.Module):
+  """Gated MLP (``gate``: 'gelu' or 'silu'): ``(gate(x Wg) * (x Wu)) Wo``; takes the place of
+  ``MlpBlock`` where the encoder's ``mlp_gate`` is set. The reference has no gated MLP."""
+
+  def __init__(self, hidden_size: int, mlp_dim: int, out_dim: Optional[int] = None,
+               dropout_rate: float = 0.0, gate: str = "gelu"):
+    super().__init__()
+    self.dropout_rate = dropout_rate
+    self.gate = check_gate(gate)
+    parts = _gated_parameters(1, hidden_size, mlp_dim, out_dim or hidden_size)
+    self.w_in, self.b_in, self.w_out, self.b_out = (nn.Parameter(p) for p in parts)
+
+  def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+    shape = x.shape
+    x3 = x.reshape(1, -1, shape[-1])
+    if self.training and self.dropout_rate > 0:
+      y = _gated_with_dropout(x3, self.w_in, self.b_in, self.w_out, self.b_out, self.gate,
+                              self.dropout_rate).reshape(*shape[:-1], -1)
+      return y if residual is None else y + residual
+    res3 = None if residual is None else residual.reshape(1, -1, residual.shape[-1])
+    y = ops.expert_gated_mlp(x3, self.w_in, self.b_in, self.w_out, self.b_out, act=self.gate,
+                             residual=res3)
+    return y.reshape(*shape[:-1], -1)
+
+
+class GatedExpertMlp(nn.Module):
+  """The gated MLPs of the experts held by this rank (see ``ExpertMlp`` for the arguments)."""
+
+  def __init__(self, num_local_experts: int, hidden_size: int, mlp_dim: int,
+               dropout_rate: float = 0.0, num_experts: Optional[int] = None,
+               first_expert: int = 0, split_rngs: bool = False, gate: str = "gelu"):
+    super().__init__()
+    self.dropout_rate = dropout_rate
+    self.gate = check_gate(gate)
+    total = num_experts or num_local_experts
+    parts = _gated_parameters(total if split_rngs else 1, hidden_size, mlp_dim, hidden_size)
+    sl = slice(first_expert, first_expert + num_local_experts)
+    self.w_in, self.b_in, self.w_out, self.b_out = (
+        nn.Parameter((t[sl] if split_rngs else t.expand(num_local_experts, *t.shape[1:])).clone())
+        for t in parts)
+    for p in (self.w_in, self.b_in, self.w_out, self.b_out):
+      p.expert_sharded = True  # sharded over the 'expert' mesh axis (dim 0)
+
+  def forward(self, x: Tensor) -> Tensor:
+    if self.training and self.dropout_rate > 0:
+      return _gated_with_dropout(x, self.w_in, self.b_in, self.w_out, self.b_out, self.gate,
+                                 self.dropout_rate)
+    return ops.expert_gated_mlp(x, self.w_in, self.b_in, self.w_out, self.b_out, act=self.gate)
+
+
+def check_gate(gate: str) -> str:
+  if gate not in ("gelu", "silu"):
+    raise ValueError(f"mlp_gate must be 'gelu' or 'silu', got {gate!r}")
+  return gate
+
+
 class MlpMoeBlock(nn.Module):
   """Sparse MoE of MLPs: tokens are regrouped into groups of ``group_size`` and each group is
   routed independently; experts are sharded over the 'expert' axis of the mesh."""
@@ -165,7 +245,7 @@ class MlpMoeBlock(nn.Module):
                dropout_rate: float = 0.0, router: Optional[KwArgs] = None,
                dtype: Optional[torch.dtype] = None,
                split_rngs: Union[bool, Iterable[str]] = False,
-               mesh: Optional[mesh_lib.Mesh] = None):
+               mesh: Optional[mesh_lib.Mesh] = None, mlp_gate: Optional[str] = None):
     super().__init__()
     self.group_size = group_size
     self.num_experts = num_experts
@@ -181,10 +261,13 @@ class MlpMoeBlock(nn.Module):
     else:
       split_params = "params" in set(split_rngs)
     self.Router = self.create_router(hidden_size, num_experts, router, dtype)
-    self.Mlp = ExpertMlp(self.num_local_experts, hidden_size, mlp_dim, dropout_rate,
-                         num_experts=num_experts,
-                         first_expert=mesh.expert_rank * self.num_local_experts,
-                         split_rngs=split_params)
+    kwargs = dict(num_experts=num_experts, split_rngs=split_params,
+                  first_expert=mesh.expert_rank * self.num_local_experts)
+    if mlp_gate is None:
+      self.Mlp = ExpertMlp(self.num_local_experts, hidden_size, mlp_dim, dropout_rate, **kwargs)
+    else:
+      self.Mlp = GatedExpertMlp(self.num_local_experts, hidden_size, mlp_dim, dropout_rate,
+                                gate=mlp_gate, **kwargs)
 
   def create_router(self, hidden_size, num_experts, router, dtype) -> nn.Module:
     kwargs = dict(num_experts=num_experts, **(router or {}))
@@ -269,14 +352,16 @@ class MultiHeadDotProductAttention(nn.Module):
 class MapHead(nn.Module):
   """Multihead attention pooling: a learned probe attends over the tokens."""
 
-  def __init__(self, hidden_size: int, mlp_dim: int, num_heads: int, qk_norm: bool = False):
+  def __init__(self, hidden_size: int, mlp_dim: int, num_heads: int, qk_norm: bool = False,
+               mlp_gate: Optional[str] = None):
     super().__init__()
     self.probe = nn.Parameter(torch.empty(1, 1, hidden_size))
     xavier_uniform_(self.probe, hidden_size, hidden_size)
     self.MultiHeadDotProductAttention = MultiHeadDotProductAttention(
         hidden_size, num_heads, normalize_qk=qk_norm)
     self.LayerNorm = LayerNorm(hidden_size)
-    self.Mlp = MlpBlock(hidden_size, mlp_dim)
+    self.Mlp = (MlpBlock(hidden_size, mlp_dim) if mlp_gate is None else
+                GatedMlpBlock(hidden_size, mlp_dim, gate=mlp_gate))
 
   def forward(self, x: Tensor) -> Tensor:
     probe = self.probe.to(x.dtype).expand(x.shape[0], -1, -1)
@@ -347,7 +432,9 @@ class AddPositionEmbs(nn.Module):
 
 
 class EncoderMoe(nn.Module):
-  """Transformer encoder; blocks listed in ``moe['layers']`` use a sparse MoE of MLPs."""
+  """Transformer encoder; blocks listed in ``moe['layers']`` use a sparse MoE of MLPs. With
+  ``mlp_gate`` ('gelu' or 'silu') the MLPs, dense and expert ones, are gated; ``moe['mlp_gate']``
+  sets the experts' apart."""
 
   DEFAULT_SINCOS2D_TEMPERATURE = 10_000.0
 
@@ -355,7 +442,8 @@ class EncoderMoe(nn.Module):
                num_heads: int, dropout_rate: float = 0.0, attention_dropout_rate: float = 0.0,
                attention_qk_norm: bool = False, moe: Optional[KwArgs] = None,
                dtype=None, position_emb: Optional[KwArgs] = None,
-               mesh: Optional[mesh_lib.Mesh] = None, moe_block_cls=None):
+               mesh: Optional[mesh_lib.Mesh] = None, moe_block_cls=None,
+               mlp_gate: Optional[str] = None):
     super().__init__()
     self.dropout_rate = dropout_rate
     self.dtype = parse_dtype(dtype)
@@ -365,7 +453,8 @@ class EncoderMoe(nn.Module):
       self.posembed_input = AddPositionEmbs(seq_len, hidden_size)
     elif name not in ("none", "sincos2d"):
       raise ValueError(f"Unsupported position embedding: {position_emb}")
-    moe_params = {"mlp_dim": mlp_dim, "dropout_rate": dropout_rate, **dict(moe or {})}
+    moe_params = {"mlp_dim": mlp_dim, "dropout_rate": dropout_rate,
+                  **({} if mlp_gate is None else {"mlp_gate": mlp_gate}), **dict(moe or {})}
     moe_layers = tuple(moe_params.pop("layers", ()))
     self.moe_layers = moe_layers
     self.num_layers = num_layers
@@ -374,8 +463,10 @@ class EncoderMoe(nn.Module):
       is_moe = block in moe_layers
       if is_moe:
         mlp = moe_block_cls(hidden_size=hidden_size, dtype=self.dtype, mesh=mesh, **moe_params)
-      else:
+      elif mlp_gate is None:
         mlp = MlpBlock(hidden_size, mlp_dim, dropout_rate=dropout_rate)
+      else:
+        mlp = GatedMlpBlock(hidden_size, mlp_dim, dropout_rate=dropout_rate, gate=mlp_gate)
       self.add_module(
           f"encoderblock_{block}",
           EncoderBlock(hidden_size, num_heads, mlp, is_moe, dropout_rate,
@@ -471,7 +562,8 @@ class VisionTransformerMoe(nn.Module):
                                     **encoder_kwargs)
     if classifier == "map":
       self.MapHead = MapHead(hidden_size, encoder["mlp_dim"], encoder["num_heads"],
-                             qk_norm=encoder.get("attention_qk_norm", False))
+                             qk_norm=encoder.get("attention_qk_norm", False),
+                             mlp_gate=encoder.get("mlp_gate"))
     feat = hidden_size
     if representation_size is not None:
       self.pre_logits = Dense(hidden_size, representation_size)

@@ -452,6 +452,57 @@ class _FusedMoeFn(torch.autograd.Function):
     return dx, dgate, dw1, db1, dw2, db2, d_res, None, None, None, None, None
 
 
+class _DispatchRowsFn(torch.autograd.Function):
+  """Rows of ``x (G, S, H)`` to the experts' buffers ``(E, G*C, H)`` (empty slots: zeros)."""
+
+  @staticmethod
+  def forward(ctx, x, expert, slot, slot_pair, capacity):
+    g, s, h = x.shape
+    e, k = slot_pair.shape[1], expert.shape[-1]
+    x = x.contiguous()
+    buf = torch.empty(e, g * capacity, h, dtype=torch.bfloat16, device=x.device)
+    gather_rows(x, slot_pair, None, base_table(buf), g, s, e, capacity, k, h)
+    ctx.save_for_backward(expert, slot)
+    ctx.dims = (g, s, e, capacity, k, h)
+    return buf
+
+  @staticmethod
+  def backward(ctx, dbuf):
+    expert, slot = ctx.saved_tensors
+    g, s, e, c, k, h = ctx.dims
+    dbuf = dbuf.contiguous()
+    dx = torch.empty(g, s, h, dtype=torch.bfloat16, device=dbuf.device)
+    combine_rows(base_table(dbuf), expert, slot, None, None, dx, g, s, e, c, k, h)
+    return dx, None, None, None, None
+
+
+class _CombineRowsFn(torch.autograd.Function):
+  """Gate-weighted sum of the experts' output rows for every item (+ residual)."""
+
+  @staticmethod
+  def forward(ctx, buf, gate, residual, expert, slot, slot_pair, capacity):
+    g, s, k = expert.shape
+    e, h = buf.shape[0], buf.shape[2]
+    buf, gate = buf.contiguous(), gate.contiguous().float()
+    residual = None if residual is None else residual.contiguous()
+    out = torch.empty(g, s, h, dtype=torch.bfloat16, device=buf.device)
+    combine_rows(base_table(buf), expert, slot, gate, residual, out, g, s, e, capacity, k, h)
+    ctx.save_for_backward(buf, gate, slot_pair)
+    ctx.dims = (g, s, e, capacity, k, h)
+    ctx.has_res = residual is not None
+    return out
+
+  @staticmethod
+  def backward(ctx, dy):
+    buf, gate, slot_pair = ctx.saved_tensors
+    g, s, e, c, k, h = ctx.dims
+    dy = dy.contiguous()
+    dbuf = torch.empty_like(buf)
+    dgate = torch.zeros(g, s, k, dtype=torch.float32, device=dy.device)
+    combine_bwd(dy, slot_pair, gate, base_table(buf), base_table(dbuf), dgate, g, s, e, c, k, h)
+    return dbuf, dgate, dy if ctx.has_res else None, None, None, None, None
+
+
 class FusedTopKDispatcher(moe_core.BaseDispatcher):
   """Top-K dispatcher for CUDA bf16 activations backed by the kernels of this module.
 
@@ -490,6 +541,15 @@ class FusedTopKDispatcher(moe_core.BaseDispatcher):
     if mlp.training and getattr(mlp, "dropout_rate", 0.0) > 0:
       out = moe_core.sparse_moe_apply(mlp, self._generic(), x)
       return out if residual is None else out + residual
+    if not hasattr(mlp, "w1"):
+      # Other MLPs than the plain two-layer one (gated ones): rows move on the kernels, the MLP is
+      # called as a module. With experts on several GPUs the generic dispatcher exchanges the rows.
+      if self.exchange.size > 1:
+        out = moe_core.sparse_moe_apply(mlp, self._generic(), x)
+        return out if residual is None else out + residual
+      buf = _DispatchRowsFn.apply(x, self.expert, self.slot, self.slot_pair, self.capacity)
+      return _CombineRowsFn.apply(mlp(buf), self.combine_weights, residual, self.expert, self.slot,
+                                  self.slot_pair, self.capacity)
     if p2p_enabled(self.exchange):
       g, s, h = x.shape
       comm = layer_comm(mlp, self.exchange, self.num_experts, g * self.capacity, h, x.device)

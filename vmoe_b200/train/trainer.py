@@ -262,6 +262,71 @@ def wrap_train_step_with_mixup(train_step_fn, *, concentration: Optional[float] 
   return new_train_step_fn
 
 
+# ------------------------------------------------------------------------------------ distillation
+class DistilledLabels:
+  """A batch's labels together with the teacher's answer to it (``losses.TopLogits``); slicing takes
+  the same examples of all of them (micro-steps)."""
+
+  def __init__(self, labels: Tensor, top):
+    self.labels, self.top = labels, top
+
+  def __getitem__(self, index) -> "DistilledLabels":
+    return DistilledLabels(self.labels[index], type(self.top)(*(t[index] for t in self.top)))
+
+
+def create_teacher(*, model_config: Mapping[str, Any], initialization: Optional[Mapping] = None,
+                   mesh: Optional[mesh_lib.Mesh] = None, device: Optional[torch.device] = None,
+                   seed: int = 0, **model_overrides) -> torch.nn.Module:
+  """A frozen model in inference mode; ``initialization`` has the kwargs of
+  ``initialize_train_state_from_checkpoint``."""
+  mesh = mesh or mesh_lib.get_mesh()
+  with torch.random.fork_rng(devices=[]):  # the same weights on every rank, and whatever was drawn before
+    torch.manual_seed(seed)
+    model = models_lib.create_model(model_config, deterministic=True, mesh=mesh, **model_overrides)
+  if device is not None:
+    model.to(device)
+  if initialization:
+    state = TrainState(model=model, optimizer=None, step=0, rngs={}, mesh=mesh)
+    initialize_train_state_from_checkpoint(state=state, mesh=mesh, **dict(initialization))
+  model.eval()
+  model.requires_grad_(False)
+  return model
+
+
+def wrap_train_step_with_distillation(train_step_fn, teacher: torch.nn.Module, *, top_k: int = 64,
+                                      temperature: float = 1.0, weight: float = 0.5,
+                                      use_rest: bool = True):
+  """The loss becomes ``(1 - weight) * loss + weight * distill_xent`` against the ``top_k`` largest logits
+  of ``teacher`` on the same images (``use_rest``: with all other classes as one more outcome, else the
+  kept classes renormalised). The images are the ones the step sees: wrap the result with mixup or
+  adversarial training, not the other way round."""
+  if not 0.0 <= weight <= 1.0:
+    raise ValueError(f"distillation weight must be in [0, 1], got {weight}")
+
+  def new_train_step_fn(state, images, labels, loss_fn, *args, **kwargs):
+    with torch.no_grad():
+      out = teacher(images)
+      logits = out[0] if isinstance(out, tuple) else out
+      if logits.shape[0] != images.shape[0]:
+        raise ValueError(f"the teacher answers {images.shape[0]} images with {logits.shape[0]} rows: "
+                         "an ensemble's members must be averaged before distillation")
+      classes = logits.shape[1]
+      top = losses_ops.top_logits(logits, min(top_k, classes), temperature=temperature)
+
+    def distilled_loss_fn(student, both: DistilledLabels):
+      if student.shape[1] != classes:
+        raise ValueError(f"the teacher has {classes} classes, the model {student.shape[1]}")
+      distance = losses_ops.distill_xent(student, both.top.values, both.top.indices,
+                                         both.top.rest if use_rest else None,
+                                         temperature=temperature)
+      return (1.0 - weight) * loss_fn(student, both.labels).float() + weight * distance
+
+    return train_step_fn(state, images, DistilledLabels(labels, top), distilled_loss_fn, *args,
+                         **kwargs)
+
+  return new_train_step_fn
+
+
 # ------------------------------------------------------------------------------------ PGD training
 def wrap_train_step_with_adversarial_attack(train_step_fn, loss_fn, *, max_epsilon: float,
                                             num_updates: int,
@@ -760,6 +825,15 @@ def train_and_evaluate(config, workdir: str, mesh: Optional[mesh_lib.Mesh] = Non
     sa = dict(config.summarize_arrays)
     summarizer = TreeSummarizer(**sa)
   step_fn = train_step
+  # ``config.distillation = {model, initialization, top_k, temperature, weight, use_rest}``: the teacher
+  # is the student's architecture unless ``model`` names another.
+  if config.get("distillation"):
+    distill = config.distillation
+    distill = distill.to_dict() if hasattr(distill, "to_dict") else dict(distill)
+    teacher = create_teacher(model_config=distill.pop("model", None) or config.model, mesh=mesh,
+                             device=device, initialization=distill.pop("initialization", None),
+                             image_size=image_size)
+    step_fn = wrap_train_step_with_distillation(step_fn, teacher, **distill)
   if config.get("adversarial"):
     step_fn = wrap_train_step_with_adversarial_attack(step_fn, train_loss_fn,
                                                       **dict(config.adversarial))

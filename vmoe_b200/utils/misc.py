@@ -184,9 +184,12 @@ def count_forward_flops(model: torch.nn.Module, *inputs) -> float:
   def dense_hook(mod, args, out):
     total[0] += 2.0 * rows_of(args[0]) * mod.weight.shape[0] * mod.weight.shape[1]
 
+  def mlp_weights(mod) -> int:  # multiply-adds per row of one (expert) MLP
+    weights = (mod.w_in, mod.w_out) if hasattr(mod, "w_in") else (mod.w1, mod.w2)
+    return sum(w[0].numel() for w in weights)
+
   def mlp_hook(mod, args, out):
-    _, m, h = mod.w1.shape
-    total[0] += 2.0 * rows_of(args[0]) * (h * m + m * mod.w2.shape[1])
+    total[0] += 2.0 * rows_of(args[0]) * mlp_weights(mod)
 
   def attn_hook(mod, args, out):
     q = args[0]
@@ -213,8 +216,7 @@ def count_forward_flops(model: torch.nn.Module, *inputs) -> float:
         rows = tokens * router.num_selected_experts
     elif getattr(router, "mu", None) is not None:
       rows = groups * e * router.mu.shape[2]
-    _, m, h = mod.Mlp.w1.shape
-    total[0] += 2.0 * rows * 2 * h * m
+    total[0] += 2.0 * rows * mlp_weights(mod.Mlp)
     dense = getattr(router, "dense", None)
     if dense is not None:
       total[0] += 2.0 * tokens * hdim * dense.weight.shape[0]
@@ -224,7 +226,7 @@ def count_forward_flops(model: torch.nn.Module, *inputs) -> float:
   for mod in model.modules():
     if isinstance(mod, vit_moe.MlpMoeBlock):
       handles.append(mod.register_forward_hook(moe_hook))
-    elif isinstance(mod, vit_moe.MlpBlock):
+    elif isinstance(mod, (vit_moe.MlpBlock, vit_moe.GatedMlpBlock)):
       handles.append(mod.register_forward_hook(mlp_hook))
     elif isinstance(mod, vit_moe.MultiHeadDotProductAttention):
       handles.append(mod.register_forward_hook(attn_hook))
