@@ -253,23 +253,6 @@ def expert_mlp(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Te
   return y if residual is None else y + residual
 
 
-def expert_gated_mlp(x: torch.Tensor, w_in: torch.Tensor, b_in: Optional[torch.Tensor],
-                     w_out: torch.Tensor, b_out: Optional[torch.Tensor], *, act: str = "gelu",
-                     residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-  """Per-expert gated MLP ``(act(x Wg^T + bg) * (x Wu^T + bu)) Wo^T + bo (+ residual)``.
-
-  ``x (E_local, rows, H)``; ``w_in (E, 2, M, H)`` holds the gate's projection in ``[:, 0]`` and the
-  other one in ``[:, 1]``, ``b_in (E, 2, M)`` their biases; ``w_out (E, O, M)``, ``b_out (E, O)``;
-  ``residual (E, rows, O)``. Biases may be None. ``act``: 'gelu' (tanh form) or 'silu'. Any number
-  of rows, also none; widths that are not multiples of 8 are zero-padded inside the call.
-  """
-  from vmoe_b200.ops import gated
-  gated.check_args(x, w_in, b_in, w_out, b_out, act, residual)
-  if _fast(x):
-    return gated.gated_mlp(x, w_in, b_in, w_out, b_out, act, residual)
-  return gated.gated_reference(x, w_in, b_in, w_out, b_out, act, residual)
-
-
 # ----------------------------------------------------------------------------------- layer norm
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                eps: float = 1e-6) -> torch.Tensor:

@@ -9,6 +9,7 @@ kernel for the gradients of both projections and their column sums, then GEMMs f
 from __future__ import annotations
 
 import ctypes
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
@@ -26,17 +27,16 @@ def _contiguous(t: torch.Tensor) -> torch.Tensor:
 def _bias(b):
   if b is None:
     return None
-  b = b.detach()
   return _contiguous(b if b.dtype in (torch.bfloat16, torch.float32) else b.float())
 
 
 def _weights(w: torch.Tensor) -> torch.Tensor:
-  return _contiguous(functional.bf16_shadow(w))
+  return _contiguous(w if w.dtype == torch.bfloat16 else functional.bf16_shadow(w))
 
 
 def _forward(x, w_in, b_in, w_out, b_out, residual, act: int, save: bool):
   """``(y, x, hidden, saved)`` with ``x`` as the kernels read it; the last two are inputs of the
-  backward pass (``saved`` is None without ``save``)."""
+  backward pass (``saved`` is None without ``save``). Called where autograd records nothing."""
   x = _contiguous(x)
   w_in, w_out, b_in, b_out = _weights(w_in), _weights(w_out), _bias(b_in), _bias(b_out)
   e, r, h = x.shape
@@ -45,21 +45,15 @@ def _forward(x, w_in, b_in, w_out, b_out, residual, act: int, save: bool):
   y = torch.empty((e, r, o), dtype=bf16, device=dev)
   hid = torch.empty((e, r, m), dtype=bf16, device=dev)
   saved = torch.empty((e, r, 2, m), dtype=bf16, device=dev) if save else None
-  g = _lib.GatedArgs()
-  g.x, g.w_in, g.w_out = x.data_ptr(), w_in.data_ptr(), w_out.data_ptr()
-  g.y, g.hid = y.data_ptr(), hid.data_ptr()
-  g.e, g.rows, g.h, g.m, g.o, g.act = e, r, h, m, o, act
-  if save:
-    g.saved = saved.data_ptr()
-  if b_in is not None:
-    g.b_in, g.b_in_bf16 = b_in.data_ptr(), b_in.dtype == bf16
-  if b_out is not None:
-    g.b_out, g.b_out_bf16 = b_out.data_ptr(), b_out.dtype == bf16
-  if residual is not None:
-    g.residual = residual.data_ptr()
-    g.res_batch_stride, g.ld_res, _ = residual.stride()
+  res_batch_stride, ld_res = residual.stride()[:2] if residual is not None else (0, 0)
+  b_out_bf16 = b_out is not None and b_out.dtype == bf16
+  ptr = _lib.ptr
+  g = _lib.GatedArgs(x.data_ptr(), w_in.data_ptr(), ptr(b_in), w_out.data_ptr(), ptr(b_out),
+                     ptr(residual), y.data_ptr(), hid.data_ptr(), ptr(saved), None, None, None, None,
+                     None, None, None, None, e, r, h, m, o, ld_res, res_batch_stride, act,
+                     b_in is not None and b_in.dtype == bf16, b_out_bf16)
   lib = _lib.lib()
-  if g.b_out_bf16:
+  if b_out_bf16:
     size = lib.vmoe_gated_scratch_bytes(ctypes.byref(g), 0)
     if size:
       scratch = torch.empty(size // 4, dtype=torch.float32, device=dev)
@@ -169,14 +163,15 @@ def gated_reference(x, w_in, b_in, w_out, b_out, act: str, residual=None):
 def check_args(x, w_in, b_in, w_out, b_out, act, residual) -> None:
   if act not in ACTIVATIONS:
     raise ValueError(f"expert_gated_mlp: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
-  if x.dim() != 3 or w_in.dim() != 4 or w_out.dim() != 3:
+  xs, ws, wos = x.shape, w_in.shape, w_out.shape
+  if len(xs) != 3 or len(ws) != 4 or len(wos) != 3:
     raise ValueError("expert_gated_mlp: x must be (E, R, H), w_in (E, 2, M, H), w_out (E, O, M); got "
-                     f"{tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
-  e, r, h = x.shape
-  m, o = w_in.shape[2], w_out.shape[1]
-  if w_in.shape != (e, 2, m, h) or w_out.shape != (e, o, m) or min(h, m, o) < 1:
+                     f"{tuple(xs)}, {tuple(ws)}, {tuple(wos)}")
+  e, r, h = xs
+  _, o, m = wos
+  if ws != (e, 2, m, h) or wos[0] != e or min(h, m, o) < 1:
     raise ValueError("expert_gated_mlp: x (E, R, H), w_in (E, 2, M, H) and w_out (E, O, M) do not fit "
-                     f"together: {tuple(x.shape)}, {tuple(w_in.shape)}, {tuple(w_out.shape)}")
+                     f"together: {tuple(xs)}, {tuple(ws)}, {tuple(wos)}")
   if residual is not None and residual.dtype != x.dtype:
     raise TypeError(f"expert_gated_mlp: residual must be {x.dtype} like x, got {residual.dtype}")
   dev = x.device
@@ -204,15 +199,32 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, act: str, residual=None) -> torch.Ten
     b_in = None if b_in is None else F.pad(b_in, (0, mp))
     b_out = None if b_out is None else F.pad(b_out, (0, op))
     residual = None if residual is None else F.pad(residual, (0, op))
-  if residual is not None and (residual.stride(2) != 1 or residual.stride(1) % 8 or
-                               residual.stride(0) % 8 or residual.data_ptr() % 16):
-    residual = residual.contiguous()
+  if residual is not None:
+    batch, row, unit = residual.stride()
+    if unit != 1 or row % 8 or batch % 8 or residual.data_ptr() % 16:
+      residual = residual.contiguous()
   if x.data_ptr() % 16:  # a view that starts inside 16 bytes
     x = x.clone()
   args = (x, w_in, b_in, w_out, b_out, residual)
-  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+  if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
     y = _GatedMlpFn.apply(*args, ACTIVATIONS[act])
   else:
     with _lib.on_device(x):
       y = _forward(*args, ACTIVATIONS[act], False)[0]
   return y[..., :o] if op else y
+
+
+def expert_gated_mlp(x: torch.Tensor, w_in: torch.Tensor, b_in: Optional[torch.Tensor],
+                     w_out: torch.Tensor, b_out: Optional[torch.Tensor], *, act: str = "gelu",
+                     residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+  """Per-expert gated MLP ``(act(x Wg^T + bg) * (x Wu^T + bu)) Wo^T + bo (+ residual)``.
+
+  ``x (E_local, rows, H)``; ``w_in (E, 2, M, H)`` holds the gate's projection in ``[:, 0]`` and the
+  other one in ``[:, 1]``, ``b_in (E, 2, M)`` their biases; ``w_out (E, O, M)``, ``b_out (E, O)``;
+  ``residual (E, rows, O)``. Biases may be None. ``act``: 'gelu' (tanh form) or 'silu'. Any number
+  of rows, also none; widths that are not multiples of 8 are zero-padded inside the call.
+  """
+  check_args(x, w_in, b_in, w_out, b_out, act, residual)
+  if functional._fast(x):
+    return gated_mlp(x, w_in, b_in, w_out, b_out, act, residual)
+  return gated_reference(x, w_in, b_in, w_out, b_out, act, residual)

@@ -167,19 +167,14 @@ class _DistillFn(torch.autograd.Function):
       x = _rows(logits)
       k = values.shape[1]
       dev = x.device
-      a = _lib.DistillArgs()
       loss = torch.empty(rows, dtype=torch.float32, device=dev)
       lib, code = _lib.lib(), _FLOAT_CODES[x.dtype]
       kept = torch.empty(lib.vmoe_distill_kept_floats(rows, n, k, code), dtype=torch.float32,
                          device=dev)
-      a.logits, a.values, a.indices = x.data_ptr(), values.data_ptr(), indices.data_ptr()
-      if rest is not None:
-        a.rest = rest.data_ptr()
-      a.loss, a.kept = loss.data_ptr(), kept.data_ptr()
-      a.rows, a.n, a.k, a.temperature = rows, n, k, temperature
-      a.ld, a.ld_values, a.ld_indices = _ld(x), _ld(values), _ld(indices)
-      a.dtype, a.values_dtype = code, _FLOAT_CODES[values.dtype]
-      a.indices_wide = indices.dtype == torch.int64
+      a = _lib.DistillArgs(x.data_ptr(), values.data_ptr(), indices.data_ptr(), _lib.ptr(rest),
+                           loss.data_ptr(), kept.data_ptr(), rows, n, k, _ld(x), _ld(values),
+                           _ld(indices), temperature, code, _FLOAT_CODES[values.dtype],
+                           indices.dtype == torch.int64)
       _lib.check(lib.vmoe_distill_fwd(ctypes.byref(a), _lib.stream_ptr()), "vmoe_distill_fwd")
       _lib.count_launch(2)
     ctx.save_for_backward(x, indices, kept)
