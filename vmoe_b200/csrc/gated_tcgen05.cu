@@ -132,6 +132,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
              const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_s,
              const __grid_constant__ CUtensorMap map_d, const GatedParams p) {
+  // The product behind this kernel may start as SMs become free: it fetches its weights and waits for
+  // these results.
+  if (MODE < 2) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -216,6 +219,53 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t full_base = PAIR ? mapa_shared(bar_full, 0) : bar_full;
+    auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int c0, int c1, int c2) {
+      if (PAIR) {
+        tma_load_3d_pair(dst, map, full, c0, c1, c2);
+      } else {
+        tma_load_3d(dst, map, full, c0, c1, c2);
+      }
+    };
+    // Announces a stage's bytes and fetches its part of B.
+    auto fill_b = [&](int st, int kt, int b, int nt) {
+      const uint32_t full = full_base + 8 * st;
+      if (!PAIR) {
+        mbar_expect_tx(full, a_stage + BSTAGE);
+      } else if (rank == 0) {
+        mbar_expect_tx(bar_full + 8 * st, 2 * (a_stage + BSTAGE));
+      }
+      const uint32_t b_dst = smem_u32(sB + st * BSTAGE);
+      const int k0 = kt * BK;
+      if (MODE == 0) {
+        if (PAIR) {
+          load(b_dst, &map_b, full, k0, nt * TN, 2 * b + static_cast<int>(rank));
+        } else {
+          load(b_dst, &map_b, full, k0, nt * TN, 2 * b);
+          load(b_dst + BSTAGE / 2, &map_b, full, k0, nt * TN, 2 * b + 1);
+        }
+      } else {
+        const int n0 = nt * TN + static_cast<int>(rank) * HALF;
+        if (!B_MN) {
+          load(b_dst, &map_b, full, k0, n0, b);
+        } else {
+#pragma unroll
+          for (int j = 0; j < B_ROWS / 64; ++j)
+            load(b_dst + j * CHUNK_BYTES, &map_b, full, n0 + 64 * j, k0, b);
+        }
+      }
+    };
+    // A plain product's B are weights, its A is what the kernel in front writes: every stage's B is on its
+    // way before that kernel is waited for.
+    int early = 0;
+    if (MODE >= 2) {
+      int b, mt, nt;
+      decode(cta, b, mt, nt);  // every CTA has a tile
+      early = min(nstage, k_tiles);
+      if (leader)
+        for (int kt = 0; kt < early; ++kt) fill_b(kt, kt, b, nt);
+      __syncwarp();
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
     for (int tile = cta; tile < num_tiles && ok; tile += ncta) {
       int b, mt, nt;
       decode(tile, b, mt, nt);
@@ -227,41 +277,11 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           break;
         }
         if (leader) {
-          const uint32_t full = full_base + 8 * stage;
-          if (!PAIR) {
-            mbar_expect_tx(full, a_stage + BSTAGE);
-          } else if (rank == 0) {
-            mbar_expect_tx(bar_full + 8 * stage, 2 * (a_stage + BSTAGE));
-          }
-          const uint32_t a_dst = smem_u32(sA + stage * a_stage);
-          const uint32_t b_dst = smem_u32(sB + stage * BSTAGE);
-          const int k0 = kt * BK;
-          auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
-            if (PAIR) {
-              tma_load_3d_pair(dst, map, full, c0, c1, c2);
-            } else {
-              tma_load_3d(dst, map, full, c0, c1, c2);
-            }
-          };
-          load(a_dst, &map_a, k0, m0, b);
-          if (MODE == 0) {
-            if (PAIR) {
-              load(b_dst, &map_b, k0, nt * TN, 2 * b + static_cast<int>(rank));
-            } else {
-              load(b_dst, &map_b, k0, nt * TN, 2 * b);
-              load(b_dst + BSTAGE / 2, &map_b, k0, nt * TN, 2 * b + 1);
-            }
-          } else {
-            const int n0 = nt * TN + static_cast<int>(rank) * HALF;
-            if (!B_MN) {
-              load(b_dst, &map_b, k0, n0, b);
-            } else {
-#pragma unroll
-              for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * CHUNK_BYTES, &map_b, n0 + 64 * j, k0, b);
-            }
-          }
+          if (early == 0) fill_b(stage, kt, b, nt);
+          load(smem_u32(sA + stage * a_stage), &map_a, full_base + 8 * stage, kt * BK, m0, b);
         }
         __syncwarp();
+        if (early > 0) --early;
         if (++stage == nstage) {
           stage = 0;
           phase ^= 1;
@@ -862,8 +882,9 @@ Shape choose_shape(int mode, int64_t e, int64_t rows, int64_t cols, int64_t k, c
   return best;
 }
 
+// after: the kernel in front in the stream is one of modes 0 and 1, and this one may start before its end.
 int launch(int mode, const Shape& s, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mh,
-           const CUtensorMap& ms, const CUtensorMap& md, GatedParams p, const DeviceInfo& info,
+           const CUtensorMap& ms, const CUtensorMap& md, GatedParams p, bool after, const DeviceInfo& info,
            cudaStream_t stream) {
   const int tm = s.pair ? 2 * BM : BM, tn = mode == 0 ? s.bn / 2 : s.bn;
   const long long tiles =
@@ -876,18 +897,27 @@ int launch(int mode, const Shape& s, const CUtensorMap& ma, const CUtensorMap& m
   const unsigned units = static_cast<unsigned>(tiles < most ? tiles : most);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cudaLaunchAttribute attr;
-  memset(&attr, 0, sizeof(attr));
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  memset(attr, 0, sizeof(attr));
+  int n = 0;
+  if (s.pair) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 2;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (after) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.gridDim = dim3(s.pair ? 2 * units : units);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = s.pair ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(mode, s), ma, mb, mh, ms, md, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1022,6 +1052,7 @@ void gemm_operands(VmoeGemmArgs* g, const void* a, int64_t lda, int64_t sa, int 
   g->split_k = 1;
 }
 
+// Called right behind the kernel that writes a.
 // out (e, rows, n) = a (e, rows, k) b^T + bias + residual, b (e, n, k) or, with b_mn, (e, k, n): on this
 // file's tiles or on the plain GEMM, whichever is estimated to be done first. bias_f32: the plain GEMM's
 // form of a bf16 bias.
@@ -1062,7 +1093,7 @@ int product(const void* a, const void* b, int b_mn, const void* bias, int bias_b
   p.k = static_cast<int>(k);
   p.m = static_cast<int>(n);
   p.batch = static_cast<int>(e);
-  return launch(mode, s, ma, mb, mh, mh, mh, p, info, stream);
+  return launch(mode, s, ma, mb, mh, mh, mh, p, true, info, stream);
 }
 
 // Pieces that a weight gradient's contraction over `rows` is cut into: few output tiles leave SMs
@@ -1184,7 +1215,7 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   p.batch = static_cast<int>(a->e);
   p.act = a->act;
   p.save = a->saved != nullptr;
-  if ((rc = launch(0, shape, ma, mb, mh, ms, ms, p, info, stream))) return rc;
+  if ((rc = launch(0, shape, ma, mb, mh, ms, ms, p, false, info, stream))) return rc;
   return product(a->hid, a->w_out, 0, a->b_out, a->b_out_bf16, a->scratch, a->residual, a->ld_res,
                  a->res_batch_stride, a->y, a->e, a->rows, a->o, a->m, info, stream);
 }
@@ -1229,8 +1260,12 @@ extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
     p.k = static_cast<int>(a->o);
     p.m = static_cast<int>(a->m);
     p.batch = static_cast<int>(a->e);
-    if ((rc = launch(1, shape, ma, mb, ms, ms, md, p, info, stream))) return rc;
+    if ((rc = launch(1, shape, ma, mb, ms, ms, md, p, false, info, stream))) return rc;
   }
+  if (a->dx && a->rows > 0 &&
+      (rc = product(a->dgu, a->w_in, 1, nullptr, 0, nullptr, nullptr, 0, 0, a->dx, a->e, a->rows, a->h,
+                    2 * a->m, info, stream)))
+    return rc;
   if (a->db_in || a->db_out) {
     SumsPart u = {sums, a->db_in, static_cast<int>((a->rows + 31) / 32),
                   a->db_in ? static_cast<int>(2 * a->m) : 0, a->db_in_mode == VMOE_GRAD_BF16,
@@ -1242,10 +1277,6 @@ extern "C" int vmoe_gated_bwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
                              256, 0, stream>>>(u, v);
     if ((rc = check_launch())) return rc;
   }
-  if (a->dx && a->rows > 0 &&
-      (rc = product(a->dgu, a->w_in, 1, nullptr, 0, nullptr, nullptr, 0, 0, a->dx, a->e, a->rows, a->h,
-                    2 * a->m, info, stream)))
-    return rc;
   if (a->dw_in && (rc = weight_gradient(a->dgu, a->x, a->e, a->rows, 2 * a->m, a->h, a->dw_in,
                                         a->dw_in_mode, pieces, stream)))
     return rc;
