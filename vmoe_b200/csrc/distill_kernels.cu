@@ -747,7 +747,7 @@ __device__ __forceinline__ int load_index(const void* p, int wide, long long i, 
 
 constexpr int ST = 128;            // threads of the forward kernels
 constexpr int FT = 256;            // threads of the backward kernel
-constexpr int ENTRIES = 64;        // kept classes whose logits stay in shared memory
+constexpr int ENTRIES = 256;       // kept classes whose logits stay in shared memory (at most)
 constexpr int MAX_SUM_PARTS = 32;  // parts of a row in the sums kernel
 
 struct DistillParams {
@@ -794,11 +794,12 @@ struct Running {
 
 // Sum of the student's exponentials over the classes that are NOT kept, per row and part: one pass
 // over the logits with a running maximum per thread. A bitmap in shared memory marks the kept classes
-// (one byte test per 8 bf16 elements). Nothing else is done here, so that a dozen small CTAs per SM,
-// each with its own loads in flight, keep HBM busy; the finish kernel is launched at once and works
+// (one byte test per 8 bf16 elements). Nothing else is done here, so that ten small CTAs per SM,
+// each with its own loads in flight, keep HBM busy (4096 rows of 21843 bf16, with the backward pass:
+// 111 us with 10 CTAs of 8 vectors per thread, 114 with 12 of 4, 116 with 8 of 8); the finish kernel is launched at once and works
 // on the kept classes until these sums are there.
 template <typename T>
-__global__ void __launch_bounds__(ST, 12)
+__global__ void __launch_bounds__(ST, 10)
 distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
   constexpr int W = Vec<T>::W;
   using Ord = Order<T>;
@@ -815,8 +816,8 @@ distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
   const int per = (lay.vectors + p.parts - 1) / p.parts;
   const int v0 = min(part * per, lay.vectors), v1 = min(v0 + per, lay.vectors);
   const uint4* xv = reinterpret_cast<const uint4*>(x + lay.head);
-  // Four vectors per thread and step; -inf past the end in the last, partial step.
-  constexpr int U = 4;
+  // Eight vectors per thread and step; -inf past the end in the last, partial step.
+  constexpr int U = 8;
   uint4 raw[U];
   const int mine = v1 - v0 - tid;  // vectors from this thread's first one on
   const int full = (v1 - v0) / (U * ST);
@@ -916,22 +917,23 @@ distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
 // One warp per row evaluates the at most k + 1 terms of the divergence in 64 bits, where the parts
 // that cancel between a student and a teacher that agree do no harm, nor in the gradient's q - p: all
 // but the student's normaliser before the sums over the other classes are waited for. stats and slopes
-// leave nothing but one exponential per class to the backward pass. The first ENTRIES kept classes
-// stay in shared memory.
+// leave nothing but one exponential per class to the backward pass. The first kept classes (`room` of
+// them, ENTRIES at most) stay in shared memory: beside the sums kernel's stream every dependent load
+// takes 2 to 3 us (37 rows of 131101 with 100 kept classes, loss and gradient: 33 us with 64 of
+// them there, 24 with all).
 template <typename T>
 __global__ void __launch_bounds__(ST)
 distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
   constexpr int ROWS = ST / 32;
-  __shared__ int at_smem[ROWS][ENTRIES];
-  __shared__ double t_smem[ROWS][ENTRIES], z_smem[ROWS][ENTRIES];
-  __shared__ double et_smem[ROWS][ENTRIES], ez_smem[ROWS][ENTRIES];
+  extern __shared__ double entry_smem[];
+  const int room = min(p.k, ENTRIES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long r = static_cast<long long>(blockIdx.x) * ROWS + warp;
   if (r >= p.rows) return;
   const int n = p.n, k = p.k;
   const T* x = logits + r * p.ld;
-  int* ent_at = at_smem[warp];
-  double *ent_t = t_smem[warp], *ent_z = z_smem[warp], *ent_et = et_smem[warp], *ent_ez = ez_smem[warp];
+  double *ent_t = entry_smem + warp * 4 * room, *ent_z = ent_t + room, *ent_et = ent_z + room, *ent_ez = ent_et + room;
+  int* ent_at = reinterpret_cast<int*>(entry_smem + ROWS * 4 * room) + warp * room;
   const float c = p.c;
   const double inv_t = 1.0 / p.temperature;
   auto load_entry = [&](int i, double& t, double& z) {
@@ -943,7 +945,7 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
     }
     return at;
   };
-  for (int i = lane; i < min(k, ENTRIES); i += 32) {
+  for (int i = lane; i < room; i += 32) {
     double t, z;
     ent_at[i] = load_entry(i, t, z);
     ent_t[i] = t;
@@ -951,7 +953,7 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
   }
   __syncwarp();
   auto class_at = [&](int i) {
-    return i < ENTRIES ? ent_at[i] : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
+    return i < room ? ent_at[i] : load_index(p.indices, p.indices_wide, r * p.ld_indices + i, n);
   };
   auto warp_max = [](double v) {
 #pragma unroll
@@ -975,7 +977,7 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
     if (repeated)  // the first entry of a class counts
       for (int j = 0; j < i; ++j)
         if (class_at(j) == at) return false;
-    if (i < ENTRIES) {
+    if (i < room) {
       t = ent_t[i];
       z = ent_z[i];
     } else {
@@ -1000,7 +1002,7 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
       const double et = part_of(t, t_max), ez = part_of(z, z_max);
       t_sum += et;
       z_sum += ez;
-      if (i < ENTRIES) {
+      if (i < room) {
         ent_et[i] = et;
         ent_ez[i] = ez;
       }
@@ -1015,7 +1017,7 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
     for (int i = lane; i < k; i += 32) {
       double t, z;
       if (!entry(i, t, z)) continue;
-      const double pt = (i < ENTRIES ? ent_et[i] : part_of(t, t_max)) * t_inv;
+      const double pt = (i < room ? ent_et[i] : part_of(t, t_max)) * t_inv;
       if (pt == 0.0) continue;
       fixed_loss += pt * ((t - t_max - t_log) - (z == -INFINITY ? z : z - z_max));
       mass += pt;
@@ -1062,8 +1064,8 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
     double t, z;
     float slope = 0.0f;
     if (entry(i, t, z) && !silent) {
-      const double et = i < ENTRIES ? ent_et[i] : part_of(t, t_max);
-      const double ez = i < ENTRIES ? ent_ez[i] : part_of(z, z_max);
+      const double et = i < room ? ent_et[i] : part_of(t, t_max);
+      const double ez = i < room ? ent_ez[i] : part_of(z, z_max);
       slope = static_cast<float>((ez == 0.0 ? 0.0 : ez * z_inv) - et * t_inv);
     }
     p.slopes[r * k + i] = slope;
@@ -1298,6 +1300,7 @@ static int distill_fwd(const VmoeDistillArgs* a, const DistillParams& p, cudaStr
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(static_cast<unsigned>((a->rows + ST / 32 - 1) / (ST / 32)));
   cfg.blockDim = dim3(ST);
+  cfg.dynamicSmemBytes = (ST / 32) * (a->k < ENTRIES ? a->k : ENTRIES) * (4 * sizeof(double) + sizeof(int));
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
