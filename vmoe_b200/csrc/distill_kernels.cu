@@ -15,6 +15,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "ptx_sm100.cuh"
@@ -920,7 +921,7 @@ distill_sums_kernel(const T* __restrict__ logits, const DistillParams p) {
 // leave nothing but one exponential per class to the backward pass. The first kept classes (`room` of
 // them, ENTRIES at most) stay in shared memory: beside the sums kernel's stream every dependent load
 // takes 2 to 3 us (37 rows of 131101 with 100 kept classes, loss and gradient: 33 us with 64 of
-// them there, 24 with all).
+// them there, 30 with all).
 template <typename T>
 __global__ void __launch_bounds__(ST)
 distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
@@ -1284,14 +1285,42 @@ extern "C" int64_t vmoe_distill_kept_floats(int64_t rows, int64_t n, int64_t k, 
   return (rows * (k + 2) + 3) / 4 * 4 + rows * 4 * distill_parts(rows, n, dtype);
 }
 
+// The finish kernel's CTAs can only join the sums' on an SM whose shared memory is set up with room for
+// them; sums alone would get little of it, and the finish kernel would wait for SMs to drain (37 rows of
+// 131101, loss and gradient: 30 us so, 20 us with a quarter set aside). More takes the L1 through which
+// the sums' loads pass: 4096 rows of 21843 take 111 us with a quarter, 117 with half, 129 with all.
+template <typename T>
+static int share_out() {
+  static std::atomic<unsigned long long> done{0};  // a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && (done.load() & bit)) return 0;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(distill_sums_kernel<T>),
+                             cudaFuncAttributePreferredSharedMemoryCarveout, 25);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(distill_finish_kernel<T>),
+                             cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) {
+    set_error("%s (code %d)", cudaGetErrorString(e), static_cast<int>(e));
+    cudaGetLastError();
+    return -4;
+  }
+  done.fetch_or(bit);
+  return 0;
+}
+
 template <typename T>
 static int distill_fwd(const VmoeDistillArgs* a, const DistillParams& p, cudaStream_t stream) {
   const T* logits = static_cast<const T*>(a->logits);
   constexpr int W = Vec<T>::W;
   const size_t smem = ((a->n / W + p.parts - 1) / p.parts + 4) * W / 8 + 8;
-  distill_sums_kernel<T><<<static_cast<unsigned>(a->rows * p.parts), ST, smem, stream>>>(logits, p);
-  const int rc = check_launch();
+  int rc = share_out<T>();
   if (rc) return rc;
+  distill_sums_kernel<T><<<static_cast<unsigned>(a->rows * p.parts), ST, smem, stream>>>(logits, p);
+  if ((rc = check_launch())) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cudaLaunchAttribute attr;
