@@ -162,7 +162,9 @@ def check_top(x, k, temperature=1.0):
   assert torch.equal(i.cpu(), want_i)
   bits = torch.int32 if x.dtype == torch.float32 else torch.int16  # torch's own gather rewrites NaN
   assert torch.equal(v.cpu().view(bits), x.cpu().contiguous().view(bits).gather(1, want_i.long()))
-  torch.testing.assert_close(rest.cpu().double(), want_rest, rtol=F32, atol=F32, equal_nan=True)
+  # `rest` is fp32: the lowest fp32 value over a temperature below 1 lies outside its range (-inf).
+  torch.testing.assert_close(rest.cpu().double(), want_rest.float().double(), rtol=F32, atol=F32,
+                             equal_nan=True)
 
 
 @gpu
@@ -200,6 +202,25 @@ def test_top_logits_kernel_of_rows_with_ties_masks_and_infinities(dtype):
   x[11, ::2] = -math.inf
   for k in (1, 20, 256):
     check_top(x, k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(257, 171), (300, 200), (700, 256), (1000, 120), (1001, 200), (2049, 250),
+                                 (3001, 171), (6001, 256)])
+def test_top_logits_kernel_of_many_kept_in_few_vectors(dtype, n, k):
+  low = torch.finfo(dtype).min
+  x = make(9, n, dtype, device="cuda")
+  x[0] = 1.5
+  x[1] = -math.inf
+  x[1, n // 2:n // 2 + 40] = 2.0     # fewer finite values than k
+  x[2, 3:] = low
+  x[3] = x[3].round()
+  x[4, 7::2] = math.nan
+  x[5, : k - 1] = math.inf
+  x[6, ::2] = -math.inf
+  x[7] = torch.where(x[7] > 0, torch.zeros_like(x[7]), -torch.zeros_like(x[7]))
+  check_top(x, k, 0.7)
 
 
 @gpu

@@ -2,12 +2,12 @@
 // with the log-sum-exp of all the others, and the divergence of a student from such a teacher
 // with its gradient. Logits are bf16, fp16 or fp32 rows of any stride and alignment.
 //
-// The two kernels that reduce a row bring it to shared memory first: one bulk asynchronous copy of
-// its whole 16-byte vectors, which needs no registers and has the whole row in flight at once; the
-// at most two partial vectors at the ends are filled element by element, padded with -inf. A
-// second pass over the row then costs no memory traffic. A row belongs to one CTA, or to a
-// cluster of 2, 4 or 8 CTAs when there are few rows or the row does not fit one (each takes a range
-// of vectors, results meet in distributed shared memory).
+// The selection brings a row to shared memory first: one bulk asynchronous copy of its whole 16-byte
+// vectors, which needs no registers and has the whole row in flight at once; the at most two partial
+// vectors at the ends are filled element by element, padded with -inf. A second pass over the row
+// then costs no memory traffic. A row belongs to one CTA, or to a cluster of 2, 4 or 8 CTAs when there
+// are few rows or the row does not fit one (each takes a range of vectors, results meet in
+// distributed shared memory). The divergence reads its rows as a stream.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -341,6 +341,9 @@ struct StagedRow {
 
 // ------------------------------------------------------------------------------- top logits
 constexpr int TOP_K_MAX = 256;
+// Elements that are ranked without a bound: 512 rows of 100 with k = 50 take 8.9 us so and 14.4 with
+// the bisection over elements, 512 rows of 1000 with k = 200 48 us and 22.
+constexpr int RANK_ALL = 256;
 
 // The k largest of the threads' maxima (found by bisection on their order keys) bound the
 // k-th largest value from below, so everything not below that bound is a candidate: somewhat more
@@ -352,6 +355,10 @@ constexpr int TOP_K_MAX = 256;
 // thread, and ranked by counting the larger ones. Candidates that lose and a sum that underflows get
 // anchors of their own, so that `rest` is right however far below the kept values it lies. Sums do not
 // depend on the order in which threads run.
+//
+// Measured: 4096 rows of 21843 bf16, k = 64: 68 us (2.6 TB/s; four rows per SM, whose 10 us are a copy of
+// 2.5 and then phases that wait for one another). 24 rows of 131101, k = 200, 8 CTAs each: 20 us, all of
+// it latency: copy, bounds, cluster joins, ranking of the kept. One row of 1000 fp32: 5 us.
 template <typename T, int DT>
 __global__ void __launch_bounds__(DT)
 top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, float c, double inv_t,
@@ -394,9 +401,40 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
   if (i < nv) m0 = Ord::largest(m0, st.row[i]);
   const uint32_t best = tid < nv ? max(Ord::key_of_largest(m0), Ord::key_of_largest(m1)) : 0u;
 
+  auto count_if = [&](auto test) {
+    int got = 0;
+    for (int j = tid; j < nv; j += DT) {
+      const uint4 q = st.row[j];
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int at = st.position(j, e);
+        if (static_cast<unsigned>(at) < static_cast<unsigned>(n))
+          got += test(Ord::key(bits_at<T>(q, e)), at) ? 1 : 0;
+      }
+    }
+    return static_cast<int>(block_reduce<DT>(static_cast<uint32_t>(got), red_u, Sum()));
+  };
+
   // Bound: at least `mine` elements have a key >= bound (0: all elements).
   uint32_t bound = 0;
-  if (__syncthreads_count(best != 0) >= mine && mine > 0) {
+  const int maxima = __syncthreads_count(best != 0);
+  if (maxima < mine + mine / 2 && mine > 0) {
+    // Too few maxima for a useful bound (they belong to single vectors): bisection over the elements, unless
+    // ranking all of them costs less.
+    if (st.elements() > RANK_ALL && st.elements() > mine + mine / 8 + 4) {
+      uint32_t hi = block_reduce<DT>(best, red_u, Max());
+      while (bound < hi) {
+        const uint32_t mid = bound + (hi - bound) / 2 + 1;
+        const int got = count_if([&](uint32_t key, int) { return key >= mid; });
+        if (got >= mine) {
+          bound = mid;
+          if (got <= mine + mine / 8 + 4) break;
+        } else {
+          hi = mid - 1;
+        }
+      }
+    }
+  } else if (mine > 0) {
     uint32_t lo = __reduce_min_sync(0xffffffffu, best ? best : 0xffffffffu);
     uint32_t hi = __reduce_max_sync(0xffffffffu, best);
     if ((tid & 31) == 0) red_range[tid >> 5] = make_uint2(lo, hi);
@@ -505,19 +543,6 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     s = near ? s0 + s1 : 0.0f;
     __syncthreads();
     if ((hot_count <= TOP_CAP && count <= TOP_CAP) || attempt == 1) break;
-    auto count_if = [&](auto test) {
-      int got = 0;
-      for (int j = tid; j < nv; j += DT) {
-        const uint4 q = st.row[j];
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const int at = st.position(j, e);
-          if (static_cast<unsigned>(at) < static_cast<unsigned>(n))
-            got += test(Ord::key(bits_at<T>(q, e)), at) ? 1 : 0;
-        }
-      }
-      return static_cast<int>(block_reduce<DT>(static_cast<uint32_t>(got), red_u, Sum()));
-    };
     uint32_t lo = bound, hi = sizeof(T) == 4 ? 0xffffffffu : 0xffffu;
     int got = TOP_CAP + 1;
     while (lo < hi && got > TOP_CAP) {
@@ -1084,8 +1109,8 @@ distill_finish_kernel(const T* __restrict__ logits, const DistillParams p) {
 }
 
 // d loss / d logits * d_loss: 2^((x - anchor) c) * factor for the classes that are not kept, the
-// saved slope for the others. One read and one write of the row; a row whose d_loss is zero (padding)
-// is zeroed without being read. Columns n .. n_pad (row padding of the gradient) get zeros.
+// saved slope for the others. One read and one write of the row (4096 rows of 21843 bf16: 59 us, 6.0 TB/s);
+// a row whose d_loss is zero (padding) is zeroed without being read. Columns n .. n_pad (row padding of the gradient) get zeros.
 template <typename T>
 __global__ void __launch_bounds__(FT)
 distill_bwd_kernel(const T* __restrict__ logits, const void* __restrict__ indices, int indices_wide,
@@ -1206,7 +1231,8 @@ int bad(const char* what) {
   return -1;
 }
 
-constexpr int kTargetCtas = 296;  // two CTAs per SM
+// Two CTAs per SM. (24 rows of 131101: 20 us with 8 CTAs for each row; 1 row of 1000 stays with one.)
+constexpr int kTargetCtas = 296;
 
 // CTAs per row: enough to give every SM two, as long as each keeps `least` vectors.
 int choose_parts(int64_t rows, int vectors, int least, int64_t target = kTargetCtas, int most = MAX_PARTS) {
@@ -1230,14 +1256,16 @@ int staged_parts(int64_t rows, int64_t n, int itemsize, int least, size_t* bytes
 template <typename T>
 int top_logits(const void* logits, int64_t rows, int64_t n, int64_t ld, int64_t k, double temperature,
                void* values, int32_t* indices, float* rest, cudaStream_t stream) {
-  size_t smem = 0;
+  size_t smem = 0;  // at first of the row's part alone
   const int parts = staged_parts(rows, n, sizeof(T), 256, &smem);
+  // 512 threads, where 256 maxima are too few to bound the k-th largest value with and the row has more
+  // vectors than that: 4096 rows of 21843 bf16 take 141 us against 943 with k = 200, but 98 against 77
+  // with k = 100; 512 rows of 1000 with k = 200 35 against 22.
+  const int threads = k + k / 2 > 256 && smem / 16 > 256 ? 512 : 256;
   const int list_offset = static_cast<int>(smem / 8);
   if (parts > 1) smem += static_cast<size_t>(parts * k * 8);
   const float c = static_cast<float>(1.4426950408889634 / temperature);
   const double inv_t = 1.0 / temperature;
-  // More threads give more maxima to bound the k-th largest value with.
-  const int threads = k > 96 ? 512 : 256;
   auto kernel = threads == 512 ? top_logits_kernel<T, 512> : top_logits_kernel<T, 256>;
   return launch_clusters(kernel, rows, parts, threads, smem, stream, static_cast<const T*>(logits),
                          static_cast<long long>(ld), static_cast<int>(n), static_cast<int>(k), c, inv_t,
