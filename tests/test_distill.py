@@ -413,3 +413,42 @@ def test_results_do_not_depend_on_the_run(n, k):
   first = step()
   for _ in range(5):
     assert all(torch.equal(a, b) for a, b in zip(first, step()))
+
+
+@gpu
+def test_second_derivatives_are_refused():
+  x = make(3, 50, torch.float32, device="cuda").requires_grad_()
+  top = losses.top_logits(make(3, 50, torch.float32, seed=4, device="cuda"), 5)
+  (grad,) = torch.autograd.grad(losses.distill_xent(x, *top).sum(), x, create_graph=True)
+  with pytest.raises(RuntimeError):
+    grad.sum().backward()
+
+
+@gpu
+def test_offsets_past_32_bits():
+  """The last rows of logits with more than 2^31 elements."""
+  n, few, copies = 21843, 500, 200
+  block = make(few, n, torch.bfloat16, device="cuda")
+  x = block.repeat(copies, 1)
+  assert x.numel() > 2 ** 31
+  small, large = losses.top_logits(block, 20), losses.top_logits(x, 20)
+  for part in (slice(None, few), slice(-few, None)):
+    assert torch.equal(small.values, large.values[part])
+    assert torch.equal(small.indices, large.indices[part])
+    # 500 * 21843 * 199 elements further on a row starts elsewhere within 16 bytes: other vectors, so
+    # its fp32 sum is added in another order.
+    torch.testing.assert_close(small.rest, large.rest[part], rtol=F32, atol=F32)
+  # Loss and gradient: rows of one CTA in both calls, so that both add in the same order.
+  block, x = block[:, :2000].contiguous(), None
+  wide = torch.empty(few * copies, n, dtype=torch.bfloat16, device="cuda")[:, :2000]
+  wide.copy_(block.repeat(copies, 1))
+  teacher = losses.top_logits(block.flip(1).contiguous(), 20)
+  found = []
+  for logits, times in ((block, 1), (wide, copies)):
+    logits = logits.detach().requires_grad_()
+    loss = losses.distill_xent(logits, *(t.repeat(times, *[1] * (t.dim() - 1)) for t in teacher))
+    (grad,) = torch.autograd.grad(loss, logits, torch.ones_like(loss))
+    found.append((loss.detach()[-few:], grad[-few:]))
+  # fp32 sums of 2000 exponentials in another split, and one rounding of the gradient to bf16.
+  torch.testing.assert_close(found[1][0], found[0][0], rtol=1e-4, atol=1e-4)
+  torch.testing.assert_close(found[1][1].float(), found[0][1].float(), rtol=2.0 ** -7, atol=1e-6)

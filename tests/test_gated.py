@@ -284,3 +284,30 @@ def test_side_stream_and_graph_replay(r):
     graph.replay()
     assert torch.equal(out[0], want[key][0])
     assert torch.equal(out[1], want[key][2]["x"]) and torch.equal(out[2], want[key][2]["w_in"])
+
+
+@gpu
+@pytest.mark.parametrize("r", [2, 60])
+def test_second_derivatives_are_refused(r):
+  t = make(1, r, 64, 96, dtype=torch.bfloat16, device="cuda")
+  x = t["x"].requires_grad_()
+  y = ops.expert_gated_mlp(x, *split(t)[1:])
+  (grad,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+  with pytest.raises(RuntimeError):
+    grad.sum().backward()
+
+
+@gpu
+def test_offsets_past_32_bits():
+  """The last rows where hidden units and factors have more than 2^31 elements."""
+  t = make(1, 64, 64, 1024, dtype=torch.bfloat16, device="cuda")
+  dy = torch.randn(1, 64, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+  want = oracle(t, "gelu", dy)
+  copies = 33000
+  x = t["x"].repeat(1, copies, 1).requires_grad_()
+  assert x.shape[1] * 1024 > 2 ** 31
+  y = ops.expert_gated_mlp(x, *split(t)[1:])
+  check(y[:, -64:], want["y"], "y")
+  (dx,) = torch.autograd.grad(y, x, dy.repeat(1, copies, 1))
+  check(dx[:, -64:], want["x"], "dx")
+  check(dx[:, :64], want["x"], "dx")

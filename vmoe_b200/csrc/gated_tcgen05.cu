@@ -609,8 +609,9 @@ gated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
           }
           if (p.sums && row0 < p.rows) {
             // Column sums of the 32 staged rows: lanes 0-15 take the even rows, 16-31 the odd ones
-            // of two columns each (rows past the end hold zeros). Written, not added: a second
-            // kernel joins the row blocks in a fixed order.
+            // of two columns each (rows past the end hold zeros), in fp32, of dg and du as rounded: the
+            // same values that dx and dw_in are made from. Written, not added: a second kernel joins
+            // the row blocks in a fixed order.
             const long long blocks = (p.rows + 31) / 32;
             const uint32_t two = lane & 15, odd = lane >> 4;
 #pragma unroll

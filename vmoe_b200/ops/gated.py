@@ -2,9 +2,10 @@
 
 ``y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wo^T + bo (+ residual)`` per expert. One kernel runs both
 projections, the activation and the product (a tcgen05 tile kernel, or a weight-streaming one for up
-to 16 rows); the output projection is the library's GEMM or the same streaming kernel. Backward: one
-kernel for the gradients of both projections and their column sums, then GEMMs for ``dx``, ``dw_in`` and
-``dw_out``. Each direction is one call into the library. The reference has no gated MLP.
+to 16 rows); the output projection runs on the same tiles, on the library's GEMM or on the streaming
+kernel. Backward (first derivatives only): one kernel for the gradients of both projections and their
+column sums, then products for ``dx``, ``dw_in`` and ``dw_out``. Each direction is one call into the
+library. The reference has no gated MLP.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from vmoe_b200.ops import _lib, functional
 
@@ -88,6 +90,7 @@ class _GatedMlpFn(torch.autograd.Function):
     return y
 
   @staticmethod
+  @once_differentiable
   def backward(ctx, dy):
     x, w_in, w_out, saved, hid = ctx.saved_tensors
     b_in, b_out = ctx.biases

@@ -17,6 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from vmoe_b200 import moe as moe_core
 from vmoe_b200.ops import _lib
@@ -467,6 +468,7 @@ class _DispatchRowsFn(torch.autograd.Function):
     return buf
 
   @staticmethod
+  @once_differentiable
   def backward(ctx, dbuf):
     expert, slot = ctx.saved_tensors
     g, s, e, c, k, h = ctx.dims
@@ -493,6 +495,7 @@ class _CombineRowsFn(torch.autograd.Function):
     return out
 
   @staticmethod
+  @once_differentiable
   def backward(ctx, dy):
     buf, gate, slot_pair = ctx.saved_tensors
     g, s, e, c, k, h = ctx.dims
@@ -548,7 +551,7 @@ class FusedTopKDispatcher(moe_core.BaseDispatcher):
         out = moe_core.sparse_moe_apply(mlp, self._generic(), x)
         return out if residual is None else out + residual
       buf = _DispatchRowsFn.apply(x, self.expert, self.slot, self.slot_pair, self.capacity)
-      return _CombineRowsFn.apply(mlp(buf), self.combine_weights, residual, self.expert, self.slot,
+      return _CombineRowsFn.apply(mlp(buf).to(x.dtype), self.combine_weights, residual, self.expert, self.slot,
                                   self.slot_pair, self.capacity)
     if p2p_enabled(self.exchange):
       g, s, h = x.shape
