@@ -356,9 +356,10 @@ constexpr int RANK_ALL = 256;
 // anchors of their own, so that `rest` is right however far below the kept values it lies. Sums do not
 // depend on the order in which threads run.
 //
-// Measured: 4096 rows of 21843 bf16, k = 64: 68 us (2.6 TB/s; four rows per SM, whose 10 us are a copy of
-// 2.5 and then phases that wait for one another). 24 rows of 131101, k = 200, 8 CTAs each: 20 us, all of
-// it latency: copy, bounds, cluster joins, ranking of the kept. One row of 1000 fp32: 5 us.
+// Measured: 4096 rows of 21843 bf16, k = 64: 68 us (2.6 TB/s; two thirds of the issue slots are used: the
+// instructions of all phases bound it, some 13 000 warp instructions per row). 24 rows of 131101, k = 200, 8 CTAs
+// each: 20 us, all of it latency: copy, bounds, cluster joins, ranking of the kept. One row of 1000
+// fp32: 5 us.
 template <typename T, int DT>
 __global__ void __launch_bounds__(DT)
 top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, float c, double inv_t,
