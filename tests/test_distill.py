@@ -224,6 +224,18 @@ def test_top_logits_kernel_of_many_kept_in_few_vectors(dtype, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [9, 12, 40, 300])
+def test_top_logits_kernel_of_negative_rows_with_lowest_masks(dtype, n):
+  # Bounds between the largest values and the masks' value are no elements, and huge.
+  for cut in (1, 2, 3, 7):
+    x = -make(10, n, dtype, seed=cut, pad=7, device="cuda").abs()
+    x[:, cut:] = torch.finfo(dtype).min
+    for k in (1, 2, 5):
+      check_top(x, k, 2.0)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_top_logits_kernel_of_wide_rows_with_ties(dtype):
   n = 50021  # several CTAs share a row
@@ -452,3 +464,30 @@ def test_offsets_past_32_bits():
   # fp32 sums of 2000 exponentials in another split, and one rounding of the gradient to bf16.
   torch.testing.assert_close(found[1][0], found[0][0], rtol=1e-4, atol=1e-4)
   torch.testing.assert_close(found[1][1].float(), found[0][1].float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e10, 1e13, 1e20, 3e30])
+def test_distill_kernel_of_huge_logits(dtype, size):
+  n, k = 700, 6
+  x = (make(6, n, dtype, device="cuda") * size).clone()
+  x[1] = -x[1].abs()
+  x[2, ::2] = -size
+  x[3] = size
+  x[4] = -size
+  x[5, 10:] = -math.inf
+  values, indices, rest = losses.top_logits(make(6, n, dtype, seed=2, device="cuda"), k)
+  x[0, indices[0].long()] += size
+  for keep_rest in (True, False):
+    z = x.clone().requires_grad_()
+    loss = losses.distill_xent(z, values, indices, rest if keep_rest else None)
+    (grad,) = torch.autograd.grad(loss.sum(), z)
+    want, want_grad = distill_oracle(x, values, indices, rest if keep_rest else None, 1.0,
+                                     torch.ones(6))
+    # The loss is fp32: half a step of it, besides fp32 sums of 700 exponentials.
+    torch.testing.assert_close(loss.detach().cpu().double(), want.float().double(), rtol=1e-5, atol=1e-4)
+    # Gradients lie in [-1, 1]: fp32 sums, one rounding to the type, and the anchor's (2^-24 of |x| c is
+    # taken back, what a product x c itself rounds is not larger than the last bit of the difference).
+    torch.testing.assert_close(grad.cpu().double(), want_grad, rtol=2.0 ** -7 if dtype == torch.bfloat16 else 1e-4,
+                               atol=1e-4)

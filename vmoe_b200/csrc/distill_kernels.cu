@@ -611,8 +611,12 @@ top_logits_kernel(const T* __restrict__ logits, long long ld, int n, int k, floa
     });
   }
   s = block_reduce<DT>(s, red_f, Sum());  // its barriers also publish sorted[]
-  if (fabsf(m) < FAR)  // the last factor takes the rounding of m c back
-    s = (s + static_cast<float>(odd_sum) * 0x1p-28f) * exp2_approx(-fmaf(m, c, -m * c));
+  if (fabsf(m) < FAR) {  // the factor takes the rounding of m c back
+    s += static_cast<float>(odd_sum) * 0x1p-28f;
+    // (A bound that is no element may be so large that this rounding passes fp32's range; no element
+    // below it leaves anything then, and 0 times infinity must not come of it.)
+    if (s != 0.0f) s *= exp2_approx(-fmaf(m, c, -m * c));
+  }
   // Adds values (each thread's own, through `each`) whose largest key is `key` to the sum; none of
   // them lies below what is in the sum already.
   auto add_at = [&](uint32_t key, auto each) {
@@ -793,14 +797,16 @@ struct DistillParams {
 };
 
 // Running sum of exponentials with the largest x so far as anchor: s * 2^-a = sum of 2^(x c) with
-// a = -m c rounded to fp32, or s = sum of 2^((x - m) c) where m lies beyond FAR.
+// a = -m c rounded to fp32, or s = sum of 2^((x - m) c) where m lies beyond FAR_SUM: rounding -m c there
+// could be off by more than the exponents that fp32 holds (c is at most 1443: off by 64 within).
+constexpr float FAR_SUM = 1e6f;
 struct Running {
   float m, a, s;
-  __device__ __forceinline__ bool far() const { return !(fabsf(m) < FAR); }
+  __device__ __forceinline__ bool far() const { return !(fabsf(m) < FAR_SUM); }
   // What a sum relative to (m0, a0) is worth relative to this anchor.
   __device__ __forceinline__ float worth(float m0, float a0, float s0, float c) const {
     if (s0 == 0.0f) return 0.0f;
-    return s0 * exp2_approx(far() || !(fabsf(m0) < FAR) ? (m0 - m) * c : a - a0);
+    return s0 * exp2_approx(far() || !(fabsf(m0) < FAR_SUM) ? (m0 - m) * c : a - a0);
   }
   __device__ __forceinline__ void raise(float top, float c) {
     if (top > m) {
