@@ -246,8 +246,9 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
 
   Entries with an index outside ``0 .. classes - 1`` (padding: -1) are left out, of a class listed
   twice the first entry counts; an example with no entry and no ``rest`` has loss and gradient 0.
-  An example whose incoming gradient is 0 gets a zero gradient whatever its logits hold. Gradients
-  flow to ``logits`` only.
+  An example whose incoming gradient is 0 gets a zero gradient whatever its logits hold. A student whose
+  logits are all -inf has no distribution: its loss is not finite. Gradients flow to ``logits`` only
+  (first derivatives, on the kernels).
   """
   temperature = _check_logits(logits, temperature, "distill_xent")
   rows, n = logits.shape
