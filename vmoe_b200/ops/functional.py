@@ -12,6 +12,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from vmoe_b200.ops import reduce
 from vmoe_b200.ops.gemm import ACT_GELU, ACT_NONE, gemm
@@ -55,6 +56,17 @@ def bf16_shadow(p: torch.Tensor) -> torch.Tensor:
     sh.copy_(p.detach())
     p._shadow_version = ver
   return sh
+
+
+def first_order(backward):
+  """``once_differentiable`` that costs nothing where no second derivative can follow: without
+  ``create_graph`` autograd calls ``backward`` with recording off."""
+  refusing = once_differentiable(backward)
+
+  def wrapped(ctx, *grads):
+    return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+  return wrapped
 
 
 def _grad_target(p: torch.Tensor):

@@ -14,7 +14,6 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from vmoe_b200.ops import _lib, functional
 
@@ -90,7 +89,7 @@ class _GatedMlpFn(torch.autograd.Function):
     return y
 
   @staticmethod
-  @once_differentiable
+  @functional.first_order
   def backward(ctx, dy):
     x, w_in, w_out, saved, hid = ctx.saved_tensors
     b_in, b_out = ctx.biases

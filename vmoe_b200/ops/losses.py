@@ -16,7 +16,6 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from vmoe_b200.ops import _lib
 from vmoe_b200.ops import functional
@@ -183,7 +182,7 @@ class _DistillFn(torch.autograd.Function):
     return loss
 
   @staticmethod
-  @once_differentiable
+  @functional.first_order
   def backward(ctx, dloss):
     x, _, _ = ctx.saved_tensors
     a = ctx.args

@@ -17,11 +17,10 @@ from typing import Optional, Tuple
 
 import torch
 import torch.distributed as dist
-from torch.autograd.function import once_differentiable
 
 from vmoe_b200 import moe as moe_core
 from vmoe_b200.ops import _lib
-from vmoe_b200.ops.functional import (_grad_target, _wgrad_split, bf16_shadow, bias_grad,
+from vmoe_b200.ops.functional import (_grad_target, _wgrad_split, bf16_shadow, bias_grad, first_order,
                                        wgrad)
 from vmoe_b200.ops.gemm import ACT_GELU, gemm
 from vmoe_b200.parallel.exchange import ExpertExchange, LOCAL_EXCHANGE
@@ -468,7 +467,7 @@ class _DispatchRowsFn(torch.autograd.Function):
     return buf
 
   @staticmethod
-  @once_differentiable
+  @first_order
   def backward(ctx, dbuf):
     expert, slot = ctx.saved_tensors
     g, s, e, c, k, h = ctx.dims
@@ -495,7 +494,7 @@ class _CombineRowsFn(torch.autograd.Function):
     return out
 
   @staticmethod
-  @once_differentiable
+  @first_order
   def backward(ctx, dy):
     buf, gate, slot_pair = ctx.saved_tensors
     g, s, e, c, k, h = ctx.dims
