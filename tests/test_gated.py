@@ -311,3 +311,18 @@ def test_offsets_past_32_bits():
   (dx,) = torch.autograd.grad(y, x, dy.repeat(1, copies, 1))
   check(dx[:, -64:], want["x"], "dx")
   check(dx[:, :64], want["x"], "dx")
+
+
+@gpu
+@pytest.mark.parametrize("e,r,h,m,o,bias,residual", [
+    (1, 17, 64, 72, None, True, True), (1, 24, 384, 1000, 200, True, False),
+    (1, 32, 520, 264, 72, False, True), (2, 31, 136, 328, None, True, True),
+    (5, 25, 72, 64, 128, True, True), (1, 32, 8, 8, None, True, False)])
+def test_rows_between_the_kernels(e, r, h, m, o, bias, residual):
+  for act in ("gelu", "silu"):
+    t = make(e, r, h, m, o, bias, residual, torch.bfloat16, device="cuda")
+    y, dy, grads = run(t, act)
+    want = oracle(t, act, dy)
+    check(y, want["y"], "y")
+    for k, g in grads.items():
+      check(g, want[k], "d" + k)

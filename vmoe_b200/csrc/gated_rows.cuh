@@ -1,14 +1,14 @@
 // Gated MLP of a few rows: the weights are read once, straight from global memory into the tensor
 // core's register fragments.
 //
-// With R <= 16 rows the work is reading the weights (2 M K and O M elements), a few microseconds of
+// With R <= 32 rows the work is reading the weights (2 M K and O M elements), a few microseconds of
 // HBM time, so what counts is how soon all of them are in flight. A CTA takes 16 hidden units (their
 // gate and their up row) or 16 outputs; its warps, and the 1, 2, 4 or 8 CTAs of a cluster when
 // there are few units, share the contraction in units of 64 elements (a 128-byte line of every row;
 // units of 32 took 12 % longer over 32 experts of 512 x 1024), and a warp has two units' loads in
 // flight. CTAs have 8 warps, or 4 when there are two CTAs for every SM anyway (32 experts x 4 rows
-// 512 -> 1024: 21 us against 28; 1 row 768 -> 2048: 9.7 us against 8.6). m16n8k16 products take 16 weight rows as A and 8 rows of x as
-// B; the contraction's order is free, so a thread's fragments of two products are 16 consecutive
+// 512 -> 1024: 21 us against 28; 1 row 768 -> 2048: 9.7 us against 8.6). m16n8k16 products take 16 weight
+// rows as A and 8 rows of x as B; the contraction's order is free, so a thread's fragments of two products are 16 consecutive
 // bytes of a weight row and of a row of x, and neither needs shared memory. Partial sums meet in
 // shared memory, then over the cluster, in a fixed order. The tile kernel's 128-row tiles, TMA
 // pipeline and TMEM would stay nearly empty here.
@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(GR_THREADS, 512 / GR_THREADS) gated_rows_kerne
   constexpr int GR_WARPS = GR_THREADS / 32;
   constexpr int G = GATED ? 2 : 1;
   constexpr int COLS = NT * 8;
+  constexpr int X_AHEAD = NT <= 2 ? GR_AHEAD : 1;  // registers for more of x's rows than 16 are not left
   __shared__ float part[GR_WARPS][G][16][COLS + 1];
   __shared__ float joined[G][16][COLS];
   // The output projection may start now: it fetches its weights and waits for these results.
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(GR_THREADS, 512 / GR_THREADS) gated_rows_kerne
   const uint4 zero = make_uint4(0, 0, 0, 0);
   bool waited = !p.after;
   for (int c0 = first; c0 * 2 < chunks; c0 += GR_AHEAD / 2 * stride) {
-    uint4 wq[GR_AHEAD][G][2], xq[GR_AHEAD][NT];
+    uint4 wq[GR_AHEAD][G][2], xq[X_AHEAD][NT];
 #pragma unroll
     for (int u = 0; u < GR_AHEAD; ++u) {
       const int k0 = (c0 + (u >> 1) * stride) * 64 + (u & 1) * 32 + t * 8;
@@ -115,23 +116,26 @@ __global__ void __launch_bounds__(GR_THREADS, 512 / GR_THREADS) gated_rows_kerne
       asm volatile("griddepcontrol.wait;" ::: "memory");
       waited = true;
     }
-#pragma unroll
-    for (int u = 0; u < GR_AHEAD; ++u) {
+    auto load_x = [&](int u, uint4 (&to)[NT]) {
       const int k0 = (c0 + (u >> 1) * stride) * 64 + (u & 1) * 32 + t * 8;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        xq[u][j] = k0 < p.k ? *reinterpret_cast<const uint4*>(xrow[j] + k0) : zero;
-    }
+        to[j] = k0 < p.k ? *reinterpret_cast<const uint4*>(xrow[j] + k0) : zero;
+    };
+#pragma unroll
+    for (int u = 0; u < X_AHEAD; ++u) load_x(u, xq[u]);
 #pragma unroll
     for (int u = 0; u < GR_AHEAD; ++u) {
+      uint4 (&x)[NT] = xq[u % X_AHEAD];
 #pragma unroll
       for (int i = 0; i < G; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const uint4 a = wq[u][i][0], b = wq[u][i][1];
-          mma_16x8x16(acc[i][j], a.x, b.x, a.y, b.y, xq[u][j].x, xq[u][j].y);
-          mma_16x8x16(acc[i][j], a.z, b.z, a.w, b.w, xq[u][j].z, xq[u][j].w);
+          mma_16x8x16(acc[i][j], a.x, b.x, a.y, b.y, x[j].x, x[j].y);
+          mma_16x8x16(acc[i][j], a.z, b.z, a.w, b.w, x[j].z, x[j].w);
         }
+      if (u + X_AHEAD < GR_AHEAD) load_x(u + X_AHEAD, x);
     }
   }
   if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // a warp without a chunk

@@ -960,8 +960,14 @@ int check_sizes(const VmoeGatedArgs* a) {
   return 0;
 }
 
-// The few-row kernel: rows of x in groups of 8.
+// The few-row kernel (rows of x in groups of 8) takes up to 16 rows, and up to 32 where the output projection
+// has so few 64-column tiles that the tile kernel would leave most SMs idle. 1 expert of 17 rows 1280 -> 5120: 24 us
+// against 36, 3 of 32 rows 1024 -> 2736: 25 against 27; but 4 of them 36 against 32 and 8 58 against 39.
+// Up to 16 rows it is never behind: 8 experts of 16 rows 36 against 38, 1 of 16 rows 1280 -> 5120 17 against 36.
 constexpr int FEW_ROWS = 16;
+bool is_few(const VmoeGatedArgs* a, const DeviceInfo& info) {
+  return a->rows <= FEW_ROWS || (a->rows <= 2 * FEW_ROWS && 3 * a->e * ((a->o + 63) / 64) <= info.sms);
+}
 
 template <int NT, bool GATED>
 int launch_rows(RowsParams p, int e, int sms, cudaStream_t stream) {
@@ -1019,8 +1025,9 @@ int few_rows(const VmoeGatedArgs* a, const DeviceInfo& info, cudaStream_t stream
   p.m = static_cast<int>(a->m);
   p.act = a->act;
   const int e = static_cast<int>(a->e);
-  int rc = a->rows <= 8 ? launch_rows<1, true>(p, e, info.sms, stream)
-                        : launch_rows<2, true>(p, e, info.sms, stream);
+  int rc = a->rows <= 8    ? launch_rows<1, true>(p, e, info.sms, stream)
+           : a->rows <= 16 ? launch_rows<2, true>(p, e, info.sms, stream)
+                           : launch_rows<4, true>(p, e, info.sms, stream);
   if (rc) return rc;
   RowsParams q;
   memset(&q, 0, sizeof(q));
@@ -1038,8 +1045,9 @@ int few_rows(const VmoeGatedArgs* a, const DeviceInfo& info, cudaStream_t stream
   q.k = static_cast<int>(a->m);
   q.m = static_cast<int>(a->o);
   q.after = 1;
-  return a->rows <= 8 ? launch_rows<1, false>(q, e, info.sms, stream)
-                      : launch_rows<2, false>(q, e, info.sms, stream);
+  return a->rows <= 8    ? launch_rows<1, false>(q, e, info.sms, stream)
+         : a->rows <= 16 ? launch_rows<2, false>(q, e, info.sms, stream)
+                         : launch_rows<4, false>(q, e, info.sms, stream);
 }
 
 void gemm_operands(VmoeGemmArgs* g, const void* a, int64_t lda, int64_t sa, int a_mn, const void* b,
@@ -1199,7 +1207,7 @@ extern "C" int vmoe_gated_fwd(const VmoeGatedArgs* a, vmoe_stream_t stream_) {
   if (a->e == 0 || a->rows == 0) return 0;
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
-  if (a->rows <= FEW_ROWS) return few_rows(a, info, stream);
+  if (is_few(a, info)) return few_rows(a, info, stream);
   CUtensorMap ma, mb, mh, ms;
   memset(&ms, 0, sizeof(ms));
   const Shape shape = choose_shape(0, a->e, a->rows, a->m, a->h, info);

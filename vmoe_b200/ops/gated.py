@@ -2,7 +2,7 @@
 
 ``y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wo^T + bo (+ residual)`` per expert. One kernel runs both
 projections, the activation and the product (a tcgen05 tile kernel, or a weight-streaming one for up
-to 16 rows); the output projection runs on the same tiles, on the library's GEMM or on the streaming
+to 16 or 32 rows); the output projection runs on the same tiles, on the library's GEMM or on the streaming
 kernel. Backward (first derivatives only): one kernel for the gradients of both projections and their
 column sums, then products for ``dx``, ``dw_in`` and ``dw_out``. Each direction is one call into the
 library. The reference has no gated MLP.
